@@ -38,11 +38,28 @@ class cn_decode_field(ctypes.Structure):
                 ("out_n", ctypes.c_int), ("width", ctypes.c_int), ("out_off", ctypes.c_int)]
 
 
+class cn_heads(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("dim", ctypes.c_int),
+                ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
+
+
+class cn_kv_cache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_exp", ctypes.c_void_p),
+                ("v_exp", ctypes.c_void_p), ("dtype", ctypes.c_int), ("heads", ctypes.c_int), ("dim", ctypes.c_int),
+                ("page", ctypes.c_int), ("pages", ctypes.c_longlong)]
+
+
+class cn_kv_batch(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_int), ("cu_tokens", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
+                ("table", ctypes.c_void_p), ("table_width", ctypes.c_int), ("table_stride", ctypes.c_longlong)]
+
+
 class ChestnutError(RuntimeError):
     pass
 
 
 _vp, _i, _ll, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_size_t
+_heads, _cache, _batch = (ctypes.POINTER(t) for t in (cn_heads, cn_kv_cache, cn_kv_batch))
 _SIGS = {
     "cn_last_error": ([], ctypes.c_char_p),
     "cn_version": ([], _i),
@@ -78,6 +95,11 @@ _SIGS = {
     "cn_decode_layout": ([ctypes.POINTER(cn_decode_field), _i, ctypes.POINTER(_i)], _i),
     "cn_decode_outputs": ([_vp, _i, _i, ctypes.POINTER(cn_decode_field), _i, _vp, _i, _vp], _i),
     "cn_decode_frame": ([_vp, ctypes.POINTER(cn_decode_field), _i, _vp], _i),
+    "cn_rope": ([_heads, _heads, _ll, _vp, _vp, _i, _i, ctypes.c_float, _vp], _i),
+    "cn_kv_write": ([_cache, _batch, _heads, _heads, _ll, _vp], _i),
+    "cn_kv_read": ([_cache, _batch, _heads, _heads, _ll, _vp], _i),
+    "cn_paged_attention": ([_cache, _batch, _heads, _heads, _ll, ctypes.c_float, _i, _i, _vp, _sz, _vp], _i),
+    "cn_paged_attention_workspace": ([_cache, _batch, _heads, _ll, ctypes.POINTER(_sz)], _i),
     "cn_device_error": ([ctypes.POINTER(_i)], _i),
     "cn_selftest_bounded_wait": ([_i, ctypes.POINTER(_i)], _i),
     "cn_dev_alloc": ([ctypes.POINTER(_vp), _sz, _i], _i),

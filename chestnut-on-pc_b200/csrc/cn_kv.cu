@@ -1,0 +1,257 @@
+// The paged K/V cache: rows written (8 bits: quantised on the way) and read back.
+//
+// A row is the dim values of one (token, cache head).  DIM / 8 lanes hold it,
+// 8 values each: a warp takes 2 rows of 128 or 4 of 64, so its loads and stores
+// are whole 128-byte lines.  8 bits: the row's largest finite |x| comes from
+// shuffles over its lanes; its exponent e is the least one with
+// amax <= 448 * 2^e (448 = 1.75 * 2^8 is e4m3's largest value), so x * 2^-e is
+// exact in f32 and the only rounding is the one to e4m3.  A power of two costs
+// nothing against amax / 448 as a scale: e4m3's step is relative, only its
+// smallest values come a binade nearer to zero, and the attention can apply it
+// to exponents.  The places of a block's tokens (sequence by binary search of
+// cu_tokens, page from the table) are worked out once, in shared memory.
+#include "cn_heads.cuh"
+
+namespace cn {
+namespace {
+
+constexpr int kKvThreads = 256;
+constexpr int kKvMaxTokens = 16;  // tokens of one block
+
+struct KvArgs {
+  BatchArgs b;
+  void *ck, *cv;  // cache
+  uint8_t *ke, *ve;
+  void *hk, *hv;  // rows [tokens][heads][dim]
+  long long k_token, k_head, v_token, v_head;
+  int heads, per_block;
+};
+
+// Sequence of token row t, or -1: the last s with cu[s] <= t, t < cu[s + 1].
+__device__ __forceinline__ int seq_of(const BatchArgs& b, int t) {
+  int lo = 0, hi = b.n_seqs;  // cu[lo] <= t < cu[hi] if t belongs to a sequence
+  if (t < b.cu[0] || t >= b.cu[hi]) return -1;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (b.cu[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// Cache row (of head 0) of token t: page * heads * page rows + row, or -1: no such
+// place (its row reads as zeros), or -2: t belongs to no sequence.
+__device__ __forceinline__ long long place_of(const KvArgs& a, long long t) {
+  const int s = seq_of(a.b, (int)t);
+  if (s < 0) return -2;
+  const int pos = a.b.lengths[s] - a.b.cu[s + 1] + (int)t;
+  if (pos < 0) return -1;
+  const int page = page_of(a.b, s, pos);
+  if (page < 0) return -1;
+  return (((long long)page * a.heads) << a.b.page_shift) + (pos & ((1 << a.b.page_shift) - 1));
+}
+
+// The largest of v over groups of N neighbouring lanes.
+template <int N>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// 8 values of a row to codes; every lane of the row gets the row's exponent byte.
+template <typename T, int LANES>
+__device__ __forceinline__ uint2 quantise8(const uint4& raw, uint32_t* byte) {
+  float x[8];
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Num<T>::unpack(w[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+    amax = fmaxf(amax, fmaxf(isfinite(f.x) ? fabsf(f.x) : 0.f, isfinite(f.y) ? fabsf(f.y) : 0.f));
+  }
+  amax = group_max<LANES>(amax);
+  // amax = 1.m * 2^k; 448 * 2^e >= amax  <=>  e >= k - 8, or k - 7 where 1.m > 1.75
+  const uint32_t bits = __float_as_uint(amax);
+  int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  e = amax > 0.f ? min(max(e, -48), 48) : 0;
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  *byte = (uint32_t)(e + 127);
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)  // x - x is 0, or NaN where x is infinite: such a value becomes NaN, not 448
+    c[i] = floats_to_codes(fmaf(x[2 * i], inv, x[2 * i] - x[2 * i]), fmaf(x[2 * i + 1], inv, x[2 * i + 1] - x[2 * i + 1]));
+  return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+}
+
+template <typename T>
+__device__ __forceinline__ float finite_limit();
+template <>
+__device__ __forceinline__ float finite_limit<__half>() { return 65504.f; }
+template <>
+__device__ __forceinline__ float finite_limit<__nv_bfloat16>() { return __uint_as_float(0x7f7f0000u); }
+
+// 8 codes to 8 values of T.
+template <typename T>
+__device__ __forceinline__ uint4 expand8(const uint2& codes, float scale) {
+  const uint32_t c[4] = {codes.x & 0xffffu, codes.x >> 16, codes.y & 0xffffu, codes.y >> 16};
+  uint32_t w[4];
+  constexpr float kMax = 3.4e38f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Num<__half>::unpack(codes_to_h2(c[i]));
+    float a = f.x * scale, b = f.y * scale;
+    // finite values beyond T's range become its largest (NaN passes: both comparisons fail)
+    const float lim = finite_limit<T>();
+    a = fabsf(a) > lim && fabsf(a) < kMax ? copysignf(lim, a) : a;
+    b = fabsf(b) > lim && fabsf(b) < kMax ? copysignf(lim, b) : b;
+    w[i] = Num<T>::pack(a, b);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// T: type of the rows.  CODED: 8-bit cache (else of type T too).  READ: cache -> rows.
+template <typename T, int DIM, bool CODED, bool READ>
+__global__ void __launch_bounds__(kKvThreads) k_kv(const KvArgs a) {
+  constexpr int LANES = DIM / 8;  // lanes of a row
+  constexpr int RPB = kKvThreads / LANES;  // rows that the block takes at a time
+  constexpr int U = 4;
+  __shared__ long long place[kKvMaxTokens];
+  pdl_trigger();
+  pdl_wait();
+  const long long t0 = (long long)blockIdx.x * a.per_block;
+  const int nt = (int)min((long long)a.per_block, a.b.tokens - t0);
+  if (threadIdx.x < nt) place[threadIdx.x] = place_of(a, t0 + threadIdx.x);
+  __syncthreads();
+  const int lane = threadIdx.x % LANES;
+  const int rows = nt * a.heads * 2;  // [token][k or v][head]
+  for (int base = 0; base < rows; base += RPB * U) {
+    uint4 x[U];
+    uint2 c[U];
+    uint32_t byte[U];
+    long long at[U];
+    T* row[U];
+    bool v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = base + u * RPB + (int)threadIdx.x / LANES;
+      at[u] = -2;
+      byte[u] = 127;
+      x[u] = make_uint4(0, 0, 0, 0);
+      c[u] = make_uint2(0, 0);
+      if (j < rows) {
+        const int t = j / (2 * a.heads), r = j - t * 2 * a.heads;
+        v[u] = r >= a.heads;
+        const int h = v[u] ? r - a.heads : r;
+        at[u] = place[t];
+        row[u] = static_cast<T*>(v[u] ? a.hv : a.hk) + (t0 + t) * (v[u] ? a.v_token : a.k_token) +
+                 h * (v[u] ? a.v_head : a.k_head) + lane * 8;
+        if (at[u] >= 0) at[u] += (long long)h << a.b.page_shift;
+        if constexpr (!READ) {
+          if (at[u] >= 0) x[u] = *reinterpret_cast<const uint4*>(row[u]);
+        } else if (at[u] >= 0) {
+          if constexpr (CODED) {
+            c[u] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 8);
+            byte[u] = (v[u] ? a.ve : a.ke)[at[u]];
+          } else {
+            x[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 8);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if constexpr (READ) {
+        if constexpr (CODED) x[u] = expand8<T>(c[u], exp_byte(byte[u]));
+        if (at[u] >= -1) *reinterpret_cast<uint4*>(row[u]) = x[u];
+      } else if constexpr (CODED) {
+        c[u] = quantise8<T, LANES>(x[u], &byte[u]);  // all lanes: it shuffles
+        if (at[u] >= 0) {
+          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 8) = c[u];
+          if (lane == 0) (v[u] ? a.ve : a.ke)[at[u]] = (uint8_t)byte[u];
+        }
+      } else if (at[u] >= 0) {
+        *reinterpret_cast<uint4*>(static_cast<T*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 8) = x[u];
+      }
+    }
+  }
+}
+
+template <typename T, bool READ>
+cudaError_t kv_launch(const KvArgs& a, int dim, bool coded, cudaStream_t s) {
+  const dim3 grid((unsigned)((a.b.tokens + a.per_block - 1) / a.per_block)), block(kKvThreads);
+  if (dim == 128)
+    return coded ? launch_ex(k_kv<T, 128, true, READ>, grid, block, 0, s, true, a)
+                 : launch_ex(k_kv<T, 128, false, READ>, grid, block, 0, s, true, a);
+  return coded ? launch_ex(k_kv<T, 64, true, READ>, grid, block, 0, s, true, a)
+               : launch_ex(k_kv<T, 64, false, READ>, grid, block, 0, s, true, a);
+}
+
+int kv_call(const char* who, bool read, const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* k,
+            const cn_heads* v, long long tokens, void* stream) {
+  int r;
+  if ((r = check_cache(who, cache)) || (r = check_batch(who, batch, cache)) || (r = check_heads(who, "k", k, tokens, read)) ||
+      (r = check_heads(who, "v", v, tokens, read)))
+    return r;
+  if (k->dtype != v->dtype || k->dtype == CN_F32 || (cache->dtype != CN_E4M3 && cache->dtype != k->dtype)) {
+    set_last_error("%s: k (dtype %d) and v (%d) are alike, f16 or bf16, and a 16-bit cache (%d) has their dtype", who,
+                   k->dtype, v->dtype, cache->dtype);
+    return CN_ERR_ARG;
+  }
+  if (k->heads != cache->heads || v->heads != cache->heads || k->dim != cache->dim || v->dim != cache->dim) {
+    set_last_error("%s: k (%d x %d), v (%d x %d) and the cache (%d x %d) differ in heads or dim", who, k->heads, k->dim,
+                   v->heads, v->dim, cache->heads, cache->dim);
+    return CN_ERR_ARG;
+  }
+  if (tokens < 0 || tokens > INT32_MAX) {
+    set_last_error("%s: %lld tokens", who, tokens);
+    return CN_ERR_ARG;
+  }
+  if (tokens == 0 || batch->n_seqs == 0) return 0;
+  DataDevice dev;
+  const void* all[] = {cache->k, cache->v, k->data, v->data, batch->cu_tokens, batch->lengths};
+  for (const void* p : all)
+    if ((r = dev.use(who, p))) return r;
+  if (batch->table_width && (r = dev.use(who, batch->table))) return r;
+  if (cache->dtype == CN_E4M3 && ((r = dev.use(who, cache->k_exp)) || (r = dev.use(who, cache->v_exp)))) return r;
+  KvArgs a;
+  a.b = batch_args(cache, batch, tokens);
+  a.ck = cache->k;
+  a.cv = cache->v;
+  a.ke = cache->k_exp;
+  a.ve = cache->v_exp;
+  a.hk = k->data;
+  a.hv = v->data;
+  a.k_token = k->token_stride;
+  a.k_head = k->head_stride;
+  a.v_token = v->token_stride;
+  a.v_head = v->head_stride;
+  a.heads = cache->heads;
+  a.per_block = tokens >= 16384 ? 16 : tokens >= 2048 ? 4 : 1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool coded = cache->dtype == CN_E4M3;
+  cudaError_t e;
+  if (k->dtype == CN_F16)
+    e = read ? kv_launch<__half, true>(a, cache->dim, coded, s) : kv_launch<__half, false>(a, cache->dim, coded, s);
+  else
+    e = read ? kv_launch<__nv_bfloat16, true>(a, cache->dim, coded, s)
+             : kv_launch<__nv_bfloat16, false>(a, cache->dim, coded, s);
+  return launch_status(who, e);
+}
+
+}  // namespace
+}  // namespace cn
+
+extern "C" int cn_kv_write(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* k, const cn_heads* v,
+                           long long tokens, void* stream) {
+  return cn::kv_call("cn_kv_write", false, cache, batch, k, v, tokens, stream);
+}
+
+extern "C" int cn_kv_read(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* k_out,
+                          const cn_heads* v_out, long long tokens, void* stream) {
+  return cn::kv_call("cn_kv_read", true, cache, batch, k_out, v_out, tokens, stream);
+}

@@ -1,0 +1,228 @@
+// How the attention over a paged cache is cut into work, shared by its kernels.
+//
+// A tile is up to ROWS query rows that read the same keys: rows of one sequence
+// and one cache head, row r = (new token r / group, query head r % group of the
+// group).  Its keys are cut into units of KEYS positions.  All units of all
+// tiles, in the order (sequence, cache head, tile, unit), are one line, and CTA
+// c of W takes the c-th equal stretch of it: sequences of any mix of lengths
+// keep every SM busy to the end, and one long context is spread over all of
+// them.  A stretch that covers a whole tile writes its rows out; a cut tile
+// leaves (unnormalised sums, maximum, sum of weights) of each part in the
+// workspace, and k_paged_merge adds the parts up in their order, so results do
+// not depend on timing.  Tiles of at most `snap` units are never cut: a cut
+// inside one moves to its start.
+// Everything is derived on the device from the batch's arrays (each CTA finds
+// its stretch with one scan), so a captured graph replays with new lengths.
+#pragma once
+#include "cn_heads.cuh"
+
+namespace cn {
+
+struct PagedArgs {
+  BatchArgs b;
+  const void* q;
+  void* out;
+  long long q_token, q_head, o_token, o_head;
+  const void *k, *v;
+  const uint8_t *k_exp, *v_exp;
+  int heads, group;     // cache heads, query heads of each
+  float scale;          // the caller's scale * log2(e)
+  int causal, window;
+  int rows_min, rows_max;  // this launch takes the sequences with rows in [rows_min, rows_max]
+  int ctas, min_units, snap;
+  struct PagedCut* cuts;   // [ctas + 1]
+  float* part_o;           // [2 * ctas][ROWS][DIM]
+  float* part_ml;          // [2 * ctas][ROWS][2]
+};
+
+// Where CTA c's stretch begins: unit `start` of the line, inside tile (seq,
+// head, tile), which covers [first, first + units).
+struct PagedCut {
+  long long start, first, total;
+  int seq, head, tile, units;
+};
+
+struct PagedSeq {
+  int tok0, n, len, past, rows, tiles;
+};
+
+template <int ROWS>
+__device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int s) {
+  PagedSeq q;
+  const long long t0 = min((long long)max(a.b.cu[s], 0), a.b.tokens);
+  const long long t1 = min((long long)max(a.b.cu[s + 1], 0), a.b.tokens);
+  q.tok0 = (int)t0;
+  q.n = (int)max(t1 - t0, 0ll);
+  const int len = max(a.b.lengths[s], 0);
+  q.past = len - q.n;
+  q.len = min(len, a.b.table_width << a.b.page_shift);
+  if (q.len < len && q.n > 0) set_dev_error(kErrPage);
+  q.rows = q.n * a.group;
+  if (q.rows < a.rows_min || q.rows > a.rows_max) q.rows = 0;
+  q.tiles = (q.rows + ROWS - 1) / ROWS;
+  return q;
+}
+
+// Keys [lo, hi) that any row of tile b sees, lo rounded down to a unit.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedSeq& q, int b, int* lo, int* hi) {
+  const int first = q.past + b * ROWS / a.group;                                // position of the first row
+  const int last = q.past + (min((b + 1) * ROWS, q.rows) - 1) / a.group;        // and of the last one
+  *hi = last < 0 ? 0 : a.causal ? min(q.len, last + 1) : q.len;
+  *lo = a.window > 0 ? max(first - a.window + 1, 0) / KEYS * KEYS : 0;
+}
+
+// Units of tile b: at least one, so that rows without keys are written too.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ int paged_units(const PagedArgs& a, const PagedSeq& q, int b) {
+  int lo, hi;
+  paged_range<ROWS, KEYS>(a, q, b, &lo, &hi);
+  return max((hi - lo + KEYS - 1) / KEYS, 1);
+}
+
+// Sum over the block; `scratch` has a long long for each warp.
+template <int THREADS>
+__device__ __forceinline__ long long block_scan(long long v, long long* scratch, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) scratch[warp] = x;
+  __syncthreads();
+  long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += scratch[w];
+    all += scratch[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + x - v;  // exclusive
+}
+
+// What a block needs to find its stretch (shared memory).
+template <int THREADS>
+struct PagedScratch {
+  long long warp_sum[THREADS / 32];
+  int seq_units[THREADS];       // units of one head of a sequence
+  long long seq_at[2], seq_each[2];
+  PagedCut cut[2];
+};
+
+// Units of one head of sequences s0 .. s0 + THREADS - 1 into sc->seq_units.  A
+// warp takes a sequence and its lanes the tiles, a thread where a sequence has
+// one tile at most (ROWS >= rows_max).
+template <int ROWS, int KEYS, int THREADS>
+__device__ __forceinline__ void paged_count(const PagedArgs& a, int s0, PagedScratch<THREADS>* sc) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int n = min(a.b.n_seqs - s0, THREADS);
+  if (a.rows_max <= ROWS) {
+    int w = 0;
+    if (tid < n) {
+      const PagedSeq q = paged_seq<ROWS>(a, s0 + tid);
+      if (q.tiles) w = paged_units<ROWS, KEYS>(a, q, 0);
+    }
+    sc->seq_units[tid] = w;
+  } else {
+    for (int i = tid >> 5; i < THREADS; i += THREADS / 32) {
+      int w = 0;
+      if (i < n) {
+        const PagedSeq q = paged_seq<ROWS>(a, s0 + i);
+        for (int b = lane; b < q.tiles; b += 32) w += paged_units<ROWS, KEYS>(a, q, b);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+      }
+      if (lane == 0) sc->seq_units[i] = w;
+    }
+  }
+  __syncthreads();
+}
+
+// The stretch of CTA `c`: sc->cut[0] where it begins, sc->cut[1] where it ends,
+// valid for all threads on return.  Called by the whole block.
+template <int ROWS, int KEYS, int THREADS>
+__device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScratch<THREADS>* sc) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  long long total = 0;
+  for (int s0 = 0; s0 < a.b.n_seqs; s0 += THREADS) {
+    long long all;
+    paged_count<ROWS, KEYS, THREADS>(a, s0, sc);
+    block_scan<THREADS>((long long)a.heads * sc->seq_units[tid], sc->warp_sum, &all);
+    total += all;
+  }
+  // CTAs that take part: each has min_units units or more
+  const long long ctas = min((long long)a.ctas, max((total + a.min_units - 1) / a.min_units, 1ll));
+  const long long u[2] = {c < ctas ? total * c / ctas : total, c + 1 < ctas ? total * (c + 1) / ctas : total};
+  if (tid < 2) {
+    PagedCut& k = sc->cut[tid];
+    k.start = k.first = k.total = total;
+    k.seq = -1;
+    k.head = k.tile = k.units = 0;
+  }
+  __syncthreads();
+  long long before = 0;
+  for (int s0 = 0; s0 < a.b.n_seqs; s0 += THREADS) {
+    if (a.b.n_seqs > THREADS) paged_count<ROWS, KEYS, THREADS>(a, s0, sc);  // else it lies there still
+    const long long w = (long long)a.heads * sc->seq_units[tid];
+    long long all;
+    const long long at = before + block_scan<THREADS>(w, sc->warp_sum, &all);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (u[i] >= at && u[i] < at + w) {  // the sequence's thread
+        sc->cut[i].seq = s0 + tid;
+        sc->seq_at[i] = at;
+        sc->seq_each[i] = sc->seq_units[tid];
+      }
+    before += all;
+    __syncthreads();  // seq_units is read by everyone before it is counted anew
+  }
+  if (tid < 64) {  // a warp for each end: the tile of its sequence
+    PagedCut& k = sc->cut[tid >> 5];
+    if (k.seq >= 0) {
+      const PagedSeq q = paged_seq<ROWS>(a, k.seq);
+      const long long rel = u[tid >> 5] - sc->seq_at[tid >> 5], each = sc->seq_each[tid >> 5];
+      const int head = (int)(rel / each);
+      const int in_head = (int)(rel - head * each);
+      int begin = 0;  // units of the head before tile b0
+      for (int b0 = 0; b0 < q.tiles; b0 += 32) {
+        const int n = b0 + lane < q.tiles ? paged_units<ROWS, KEYS>(a, q, b0 + lane) : 0;
+        int x = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
+        }
+        const bool here = in_head >= begin + x - n && in_head < begin + x;
+        if (here) {
+          k.head = head;
+          k.tile = b0 + lane;
+          k.first = sc->seq_at[tid >> 5] + head * each + begin + x - n;
+          k.units = n;
+          k.start = n <= a.snap ? k.first : u[tid >> 5];
+        }
+        if (__any_sync(0xffffffffu, here)) break;
+        begin += __shfl_sync(0xffffffffu, x, 31);
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// The tile behind (s, head, b); false at the end of the line.
+template <int ROWS>
+__device__ __forceinline__ bool paged_next(const PagedArgs& a, PagedSeq* q, int* s, int* head, int* b) {
+  if (++*b < q->tiles) return true;
+  *b = 0;
+  if (++*head < a.heads) return true;
+  *head = 0;
+  while (++*s < a.b.n_seqs) {
+    *q = paged_seq<ROWS>(a, *s);
+    if (q->tiles) return true;
+  }
+  return false;
+}
+
+}  // namespace cn

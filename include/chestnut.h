@@ -32,6 +32,10 @@
  *                         (parse_model_outputs.py:1-120: parse_mdn,
  *                         parse_binary_crossentropy,
  *                         parse_categorical_crossentropy), on the GPU
+ *
+ * Temporal-context operators (no counterpart in the reference, whose only past
+ * is the sampled feature queue): cn_rope, cn_kv_write, cn_kv_read,
+ * cn_paged_attention.
  */
 #ifndef CHESTNUT_H
 #define CHESTNUT_H
@@ -215,6 +219,108 @@ int cn_decode_outputs(const float* raw, int batch, int raw_stride, const cn_deco
  * cn_run_frame_device) and copy the decoded values to host f32
  * [batch][out_len], out_len from cn_decode_layout.  Synchronous. */
 int cn_decode_frame(cn_engine* e, const cn_decode_field* fields, int n_fields, float* host_out);
+
+/* ---- temporal context: rotary positions, paged K/V cache, attention ------
+ * For clips whose past is longer than the frame's own attention holds (96
+ * tokens): the K and V rows of past tokens stay in pages of a cache that many
+ * clips share, and the tokens of a new frame (one, a few, or a whole first
+ * prompt) attend to them.  All pointers are device memory of one GPU, and the
+ * calls run on that GPU's stream whatever the current device is; every call
+ * only queues work and can be captured into a CUDA graph.  A pointer that is
+ * not device memory, or lies on another GPU than the call's first one, is
+ * refused. */
+#define CN_F16 0
+#define CN_BF16 1
+#define CN_F32 2
+#define CN_E4M3 3
+
+/* Rows [tokens][heads][dim]: dim values lie side by side, tokens and heads at
+ * any stride (elements, not negative), so a view of a packed q|k|v product or a
+ * [heads][tokens][dim] layout needs no copy.  data and both strides are
+ * multiples of 16 bytes. */
+typedef struct cn_heads {
+  void* data;
+  int dtype;  /* CN_F16, CN_BF16 (cn_rope also CN_F32) */
+  int heads, dim;
+  long long token_stride, head_stride;
+} cn_heads;
+
+/* The cache: k and v [pages][heads][page][dim], contiguous; page (rows of a
+ * page) 16, 32, 64, 128 or 256; dim 64 or 128.  CN_E4M3 holds 8 bits a value
+ * and one power of two a row: k_exp and v_exp, u8 [pages][heads][page], hold
+ * the row's exponent + 127, and a value is its code times 2^(byte - 127).  All
+ * 16-byte aligned.  CN_F16 / CN_BF16: k_exp = v_exp = NULL. */
+typedef struct cn_kv_cache {
+  void *k, *v;
+  uint8_t *k_exp, *v_exp;
+  int dtype, heads, dim, page;
+  long long pages;
+} cn_kv_cache;
+
+/* A batch of sequences with new tokens.  Sequence s owns token rows
+ * [cu_tokens[s], cu_tokens[s+1]) (i32 [n_seqs + 1], ascending); its context
+ * holds lengths[s] tokens, the new ones last, so new token i of n has position
+ * lengths[s] - n + i; position p lies in row p % page of page
+ * table[s * table_stride + p / page].  Token rows behind cu_tokens[n_seqs] (or
+ * before cu_tokens[0]) belong to no sequence: nothing is read from them and
+ * nothing written to them.  A negative position (lengths[s] < n) has no row:
+ * it is not written, reads back as zeros and attends to nothing.  These arrays
+ * are read on the device; a page outside the cache, or a position past
+ * table_width pages, is skipped (reads give zeros) and sets the device error
+ * word to 6 (cn_device_error). */
+typedef struct cn_kv_batch {
+  int n_seqs;
+  const int *cu_tokens, *lengths, *table;
+  int table_width;
+  long long table_stride;
+} cn_kv_batch;
+
+/* Rotary positions: turns the first rot_dim values of every head of x by its
+ * token's position and writes out (x itself, or memory that does not overlap
+ * it); values behind rot_dim are copied.  Pair i of a token at position p is
+ * turned by the angle p * inv_freq[i] (reduced in 64 bits, so far positions
+ * keep their phase) and multiplied by `magnitude`:
+ *   a' = magnitude (a cos - b sin),  b' = magnitude (b cos + a sin),
+ * with (a, b) = values (i, i + rot_dim/2), or (2i, 2i + 1) if `interleaved`.
+ * positions i64 [tokens]; inv_freq f64 [rot_dim/2], radians a token (a scaled
+ * context is scaled there).  rot_dim even, <= dim; dim % 8 == 0, <= 256; x and
+ * out alike in dtype, heads and dim.  Arithmetic in f32, rounded once. */
+int cn_rope(const cn_heads* x, const cn_heads* out, long long tokens, const long long* positions,
+            const double* inv_freq, int rot_dim, int interleaved, float magnitude, void* stream);
+/* Writes the new tokens' k and v rows into their places of the cache.  k and v
+ * have the cache's heads and dim.  A CN_F16 / CN_BF16 cache takes rows of its
+ * own dtype as they are.  CN_E4M3: with amax the largest finite |x| of a row,
+ * the row's exponent is the least e in [-48, 48] with amax <= 448 * 2^e (0 for
+ * a row of zeros), its codes x * 2^-e to the nearest e4m3, ties to even, beyond
+ * 448 to 448; NaN and infinities become NaN.  Two tokens with the same place
+ * (a page that occurs twice) are the caller's error: what that place then holds
+ * is not defined. */
+int cn_kv_write(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* k, const cn_heads* v,
+                long long tokens, void* stream);
+/* The inverse: reads the rows of the batch's new tokens back (all of a context
+ * when its length is its token count), rounded to the outputs' dtype; finite
+ * values beyond its range become its largest.  A CN_F16 / CN_BF16 cache is read
+ * in its own dtype. */
+int cn_kv_read(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* k_out, const cn_heads* v_out,
+               long long tokens, void* stream);
+/* Attention of the new tokens' queries over their sequences' contexts, which
+ * hold the new tokens already (cn_kv_write before it):
+ *   out[i] = sum_j w_ij v_j,  w_i = softmax over the visible j of scale * q_i . k_j
+ * Visible to the token at position p: every j < lengths[s], if `causal` j <= p
+ * only, and with window > 0 (causal only) j > p - window only.  A row that sees
+ * nothing is zeros, and what is not visible has no influence, whatever its value.
+ * Query head h reads cache head h / (q.heads / cache.heads).  q and out alike in
+ * dtype (CN_F16 or CN_BF16, the cache's own unless that is CN_E4M3), heads and
+ * dim; out may be q.  Statistics and sums in f32, the weights enter the product
+ * with V in 16 bits.  workspace: cn_paged_attention_workspace() bytes, 256-byte
+ * aligned, its content of no matter before and after a call; calls that may run
+ * at the same time need one each.  Results do not depend on timing. */
+int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q, const cn_heads* out,
+                       long long tokens, float scale, int causal, int window, void* workspace,
+                       size_t workspace_bytes, void* stream);
+/* Bytes that cn_paged_attention needs for these arguments (only their sizes are read). */
+int cn_paged_attention_workspace(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
+                                 long long tokens, size_t* bytes);
 
 /* Read (and clear) the device error word. */
 int cn_device_error(int* code);
