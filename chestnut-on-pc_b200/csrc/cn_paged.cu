@@ -1,5 +1,5 @@
 // Attention of new tokens over the paged cache: the kernel for sequences of few
-// query rows, the merge of cut tiles, and the entry point.
+// query rows, and the merge of cut tiles.
 //
 // k_paged_few.  One token (or a few) of a sequence against its whole context
 // reads K and V once and computes little with them: it is bound by HBM.  What
@@ -519,151 +519,5 @@ __global__ void __launch_bounds__(RPB * 32) k_paged_merge(const PagedArgs a) {
   }
 }
 
-// Workspace of one launch: the cuts, then the parts.
-struct PagedSpace {
-  size_t o, ml, bytes;
-};
-PagedSpace paged_space(int ctas, int rows, int dim) {
-  PagedSpace s;
-  s.o = ((size_t)(ctas + 1) * sizeof(PagedCut) + 255) / 256 * 256;
-  s.ml = s.o + (size_t)2 * ctas * rows * dim * 4;
-  s.bytes = s.ml + ((size_t)2 * ctas * rows * 2 * 4 + 255) / 256 * 256;
-  return s;
-}
-
-int sm_count(int dev) {
-  static int count[64];
-  if (dev < 0 || dev >= 64) return 148;
-  if (!count[dev]) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
-      cudaGetLastError();
-      return 148;
-    }
-    count[dev] = n;
-  }
-  return count[dev];
-}
-
-constexpr int kFewCtas = 2 * 148;  // two CTAs an SM
-
-template <typename T, int DIM, bool CODED>
-cudaError_t few_launch(const PagedArgs& a, bool merge, int dev, cudaStream_t s) {
-  static unsigned long long ready = 0;
-  if (dev >= 64 || !(ready & (1ull << dev))) {
-    const cudaError_t e = cudaFuncSetAttribute(k_paged_few<T, DIM, CODED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)Few<DIM, CODED>::Smem);
-    if (e != cudaSuccess) return e;
-    if (dev < 64) ready |= 1ull << dev;
-  }
-  cudaError_t e = launch_ex(k_paged_few<T, DIM, CODED>, dim3(a.ctas), dim3(kFewThreads), Few<DIM, CODED>::Smem, s, true, a);
-  if (e == cudaSuccess && merge)
-    e = launch_ex(k_paged_merge<T, DIM, kFewRows, 4>, dim3(a.ctas - 1, kFewRows / 4), dim3(128), 0, s, true, a);
-  return e;
-}
-
-template <typename T>
-cudaError_t few_dispatch(const PagedArgs& a, int dim, bool coded, bool merge, int dev, cudaStream_t s) {
-  if (dim == 128)
-    return coded ? few_launch<T, 128, true>(a, merge, dev, s) : few_launch<T, 128, false>(a, merge, dev, s);
-  return coded ? few_launch<T, 64, true>(a, merge, dev, s) : few_launch<T, 64, false>(a, merge, dev, s);
-}
-
-int paged_check(const char* who, const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
-                long long tokens) {
-  int r;
-  if ((r = check_cache(who, cache)) || (r = check_batch(who, batch, cache)) || (r = check_heads(who, "q", q, tokens, false)))
-    return r;
-  if (q->dtype == CN_F32 || (cache->dtype != CN_E4M3 && cache->dtype != q->dtype)) {
-    set_last_error("%s: q has dtype %d, the cache %d (q f16 or bf16, a 16-bit cache the same)", who, q->dtype, cache->dtype);
-    return CN_ERR_ARG;
-  }
-  if (q->dim != cache->dim || q->heads % cache->heads) {
-    set_last_error("%s: %d query heads of %d values over %d cache heads of %d", who, q->heads, q->dim, cache->heads,
-                   cache->dim);
-    return CN_ERR_ARG;
-  }
-  if (tokens < 0 || tokens * (q->heads / cache->heads) > (1ll << 30)) {
-    set_last_error("%s: %lld tokens (tokens x query heads of a cache head: at most 2^30)", who, tokens);
-    return CN_ERR_ARG;
-  }
-  return 0;
-}
-
 }  // namespace
 }  // namespace cn
-
-extern "C" int cn_paged_attention_workspace(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
-                                            long long tokens, size_t* bytes) {
-  using namespace cn;
-  const char* who = "cn_paged_attention_workspace";
-  if (!bytes) {
-    set_last_error("%s: bytes is NULL", who);
-    return CN_ERR_ARG;
-  }
-  const int r = paged_check(who, cache, batch, q, tokens);
-  if (r) return r;
-  *bytes = paged_space(kFewCtas, kFewRows, cache->dim).bytes;
-  return 0;
-}
-
-extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
-                                  const cn_heads* out, long long tokens, float scale, int causal, int window,
-                                  void* workspace, size_t workspace_bytes, void* stream) {
-  using namespace cn;
-  const char* who = "cn_paged_attention";
-  int r = paged_check(who, cache, batch, q, tokens);
-  if (r || (r = check_heads(who, "out", out, tokens, true))) return r;
-  if (out->dtype != q->dtype || out->heads != q->heads || out->dim != q->dim) {
-    set_last_error("%s: q and out differ in dtype, heads or dim", who);
-    return CN_ERR_ARG;
-  }
-  if (window < 0 || (window > 0 && !causal)) {
-    set_last_error("%s: window %d (a window needs causal)", who, window);
-    return CN_ERR_ARG;
-  }
-  const PagedSpace sp = paged_space(kFewCtas, kFewRows, cache->dim);
-  if (tokens > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < sp.bytes)) {
-    set_last_error("%s: workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", who, sp.bytes, workspace_bytes);
-    return CN_ERR_ARG;
-  }
-  if (tokens == 0 || batch->n_seqs == 0) return 0;
-  DataDevice dev;
-  const void* all[] = {cache->k, cache->v, q->data, out->data, batch->cu_tokens, batch->lengths, workspace};
-  for (const void* p : all)
-    if ((r = dev.use(who, p))) return r;
-  if (batch->table_width && (r = dev.use(who, batch->table))) return r;
-  const bool coded = cache->dtype == CN_E4M3;
-  if (coded && ((r = dev.use(who, cache->k_exp)) || (r = dev.use(who, cache->v_exp)))) return r;
-  PagedArgs a;
-  a.b = batch_args(cache, batch, tokens);
-  a.q = q->data;
-  a.out = out->data;
-  a.q_token = q->token_stride;
-  a.q_head = q->head_stride;
-  a.o_token = out->token_stride;
-  a.o_head = out->head_stride;
-  a.k = cache->k;
-  a.v = cache->v;
-  a.k_exp = cache->k_exp;
-  a.v_exp = cache->v_exp;
-  a.heads = cache->heads;
-  a.group = q->heads / cache->heads;
-  a.scale = scale * 1.44269504088896340736f;
-  a.causal = causal != 0;
-  a.window = window;
-  a.rows_min = 1;
-  a.rows_max = INT32_MAX;
-  a.ctas = min(2 * sm_count(dev.device()), kFewCtas);
-  a.min_units = 4;
-  a.snap = 4;
-  uint8_t* w = static_cast<uint8_t*>(workspace);
-  a.cuts = reinterpret_cast<PagedCut*>(w);
-  a.part_o = reinterpret_cast<float*>(w + sp.o);
-  a.part_ml = reinterpret_cast<float*>(w + sp.ml);
-  // contexts that fit into `snap` units are never cut: nothing to merge
-  const bool merge = (long long)batch->table_width * cache->page > (long long)a.snap * kFewKeys;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return launch_status(who, q->dtype == CN_F16 ? few_dispatch<__half>(a, cache->dim, coded, merge, dev.device(), s)
-                                               : few_dispatch<__nv_bfloat16>(a, cache->dim, coded, merge, dev.device(), s));
-}

@@ -1,0 +1,232 @@
+// Attention over the paged cache: choice of the launches, workspace, entry points.
+#include <cmath>
+
+#include "cn_paged.cuh"
+
+namespace cn {
+namespace {
+
+// Workspace of one launch: the cuts, then the parts.
+struct PagedSpace {
+  size_t o, ml, bytes;
+};
+PagedSpace paged_space(int ctas, int rows, int dim) {
+  PagedSpace s;
+  s.o = ((size_t)(ctas + 1) * sizeof(PagedCut) + 255) / 256 * 256;
+  s.ml = s.o + (size_t)2 * ctas * rows * dim * 4;
+  s.bytes = s.ml + ((size_t)2 * ctas * rows * 2 * 4 + 255) / 256 * 256;
+  return s;
+}
+
+int sm_count(int dev) {
+  static int count[64];
+  if (dev < 0 || dev >= 64) return 148;
+  if (!count[dev]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      return 148;
+    }
+    count[dev] = n;
+  }
+  return count[dev];
+}
+
+constexpr int kFewCtas = 2 * 148;  // two CTAs an SM
+
+constexpr int kManyCtas = 148;
+
+template <typename T, int DIM, bool CODED>
+cudaError_t few_launch(const PagedArgs& a, bool merge, int dev, cudaStream_t s) {
+  static unsigned long long ready = 0;
+  if (dev >= 64 || !(ready & (1ull << dev))) {
+    const cudaError_t e = cudaFuncSetAttribute(k_paged_few<T, DIM, CODED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)Few<DIM, CODED>::Smem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready |= 1ull << dev;
+  }
+  cudaError_t e = launch_ex(k_paged_few<T, DIM, CODED>, dim3(a.ctas), dim3(kFewThreads), Few<DIM, CODED>::Smem, s, true, a);
+  if (e == cudaSuccess && merge)
+    e = launch_ex(k_paged_merge<T, DIM, kFewRows, 4>, dim3(a.ctas - 1, kFewRows / 4), dim3(128), 0, s, true, a);
+  return e;
+}
+
+template <typename T, int DIM, bool CODED>
+cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, bool merge, int dev,
+                        cudaStream_t s) {
+  static unsigned long long ready = 0;
+  if (dev >= 64 || !(ready & (1ull << dev))) {
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, k_paged_many<T, DIM, CODED>);
+    // the warpgroups share out 4 x 128 registers: a block that is launched with fewer would wait for ever
+    if (e == cudaSuccess && at.numRegs != 128) e = cudaErrorInvalidKernelImage;
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_paged_many<T, DIM, CODED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)Many<DIM>::Smem);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) ready |= 1ull << dev;
+  }
+  cudaError_t e = launch_ex(k_paged_many<T, DIM, CODED>, dim3(a.ctas), dim3(kManyThreads), Many<DIM>::Smem, s, true, tk, tv, a);
+  if (e == cudaSuccess && merge)
+    e = launch_ex(k_paged_merge<T, DIM, kManyRows, 8>, dim3(a.ctas - 1, kManyRows / 8), dim3(256), 0, s, true, a);
+  return e;
+}
+
+// One call: the launches for few and for many rows (each where it may find work).
+struct PagedCall {
+  PagedArgs few, many;
+  bool do_few, do_many, merge_few, merge_many;
+  CUtensorMap tk, tv;
+};
+
+template <typename T, int DIM, bool CODED>
+cudaError_t paged_launch(const PagedCall& c, int dev, cudaStream_t s) {
+  cudaError_t e = cudaSuccess;
+  if (c.do_few) e = few_launch<T, DIM, CODED>(c.few, c.merge_few, dev, s);
+  if (e == cudaSuccess && c.do_many) e = many_launch<T, DIM, CODED>(c.many, c.tk, c.tv, c.merge_many, dev, s);
+  return e;
+}
+
+template <typename T>
+cudaError_t paged_dispatch(const PagedCall& c, int dim, bool coded, int dev, cudaStream_t s) {
+  if (dim == 128) return coded ? paged_launch<T, 128, true>(c, dev, s) : paged_launch<T, 128, false>(c, dev, s);
+  return coded ? paged_launch<T, 64, true>(c, dev, s) : paged_launch<T, 64, false>(c, dev, s);
+}
+
+// A 16-bit cache as [pages][heads * page rows][dim], boxes of up to 128 rows of a page x 64 values.
+int paged_map(CUtensorMap* m, const cn_kv_cache* c, const void* base) {
+  const uint64_t d[3] = {(uint64_t)c->dim, (uint64_t)c->heads * c->page, (uint64_t)c->pages};
+  const uint64_t st[2] = {(uint64_t)c->dim * 2, (uint64_t)c->heads * c->page * c->dim * 2};
+  const uint32_t b[3] = {64, (uint32_t)(c->page < kManyKeys ? c->page : kManyKeys), 1};
+  return encode(m, c->dtype == CN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, d,
+                st, b, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+int paged_check(const char* who, const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
+                long long tokens) {
+  int r;
+  if ((r = check_cache(who, cache)) || (r = check_batch(who, batch, cache)) || (r = check_heads(who, "q", q, tokens, false)))
+    return r;
+  if (q->dtype == CN_F32 || (cache->dtype != CN_E4M3 && cache->dtype != q->dtype)) {
+    set_last_error("%s: q has dtype %d, the cache %d (q f16 or bf16, a 16-bit cache the same)", who, q->dtype, cache->dtype);
+    return CN_ERR_ARG;
+  }
+  if (q->dim != cache->dim || q->heads % cache->heads) {
+    set_last_error("%s: %d query heads of %d values over %d cache heads of %d", who, q->heads, q->dim, cache->heads,
+                   cache->dim);
+    return CN_ERR_ARG;
+  }
+  if (tokens < 0 || tokens * (q->heads / cache->heads) > (1ll << 30)) {
+    set_last_error("%s: %lld tokens (tokens x query heads of a cache head: at most 2^30)", who, tokens);
+    return CN_ERR_ARG;
+  }
+  return 0;
+}
+
+}  // namespace
+}  // namespace cn
+
+extern "C" int cn_paged_attention_workspace(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
+                                            long long tokens, size_t* bytes) {
+  using namespace cn;
+  const char* who = "cn_paged_attention_workspace";
+  if (!bytes) {
+    set_last_error("%s: bytes is NULL", who);
+    return CN_ERR_ARG;
+  }
+  const int r = paged_check(who, cache, batch, q, tokens);
+  if (r) return r;
+  *bytes = paged_space(kFewCtas, kFewRows, cache->dim).bytes + paged_space(kManyCtas, kManyRows, cache->dim).bytes;
+  return 0;
+}
+
+extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
+                                  const cn_heads* out, long long tokens, float scale, int causal, int window,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace cn;
+  const char* who = "cn_paged_attention";
+  int r = paged_check(who, cache, batch, q, tokens);
+  if (r || (r = check_heads(who, "out", out, tokens, true))) return r;
+  if (out->dtype != q->dtype || out->heads != q->heads || out->dim != q->dim) {
+    set_last_error("%s: q and out differ in dtype, heads or dim", who);
+    return CN_ERR_ARG;
+  }
+  if (window < 0 || (window > 0 && !causal)) {
+    set_last_error("%s: window %d (a window needs causal)", who, window);
+    return CN_ERR_ARG;
+  }
+  if (!(scale > 0.f) || std::isinf(scale)) {
+    set_last_error("%s: scale %g (positive and finite)", who, (double)scale);
+    return CN_ERR_ARG;
+  }
+  const PagedSpace few = paged_space(kFewCtas, kFewRows, cache->dim), many = paged_space(kManyCtas, kManyRows, cache->dim);
+  if (tokens > 0 &&
+      (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256 || workspace_bytes < few.bytes + many.bytes)) {
+    set_last_error("%s: workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", who, few.bytes + many.bytes,
+                   workspace_bytes);
+    return CN_ERR_ARG;
+  }
+  if (tokens == 0 || batch->n_seqs == 0) return 0;
+  DataDevice dev;
+  const void* all[] = {cache->k, cache->v, q->data, out->data, batch->cu_tokens, batch->lengths, workspace};
+  for (const void* p : all)
+    if ((r = dev.use(who, p))) return r;
+  if (batch->table_width && (r = dev.use(who, batch->table))) return r;
+  const bool coded = cache->dtype == CN_E4M3;
+  if (coded && ((r = dev.use(who, cache->k_exp)) || (r = dev.use(who, cache->v_exp)))) return r;
+  PagedArgs a;
+  a.b = batch_args(cache, batch, tokens);
+  a.q = q->data;
+  a.out = out->data;
+  a.q_token = q->token_stride;
+  a.q_head = q->head_stride;
+  a.o_token = out->token_stride;
+  a.o_head = out->head_stride;
+  a.k = cache->k;
+  a.v = cache->v;
+  a.k_exp = cache->k_exp;
+  a.v_exp = cache->v_exp;
+  a.heads = cache->heads;
+  a.group = q->heads / cache->heads;
+  a.scale = scale * 1.44269504088896340736f;
+  a.causal = causal != 0;
+  a.window = window;
+  // Sequences of up to 16 rows go to the kernel for few rows, the others to the
+  // tensor-core one.  How long each is, only the device knows; a launch that
+  // cannot find work is left out, one that may not find any costs ~3 us.
+  const long long rows = tokens * a.group;
+  const bool steps = tokens <= batch->n_seqs && a.group <= kFewRows;  // a token a sequence
+  PagedCall c;
+  memset(&c, 0, sizeof(c));
+  c.do_few = batch->n_seqs > 1 ? a.group <= kFewRows : rows <= kFewRows;
+  c.do_many = !(steps || rows <= kFewRows);
+  uint8_t* w = static_cast<uint8_t*>(workspace);
+  const long long cap = (long long)batch->table_width * cache->page;
+  if (c.do_few) {
+    PagedArgs& f = c.few = a;
+    f.rows_min = 1;
+    f.rows_max = c.do_many ? kFewRows : INT32_MAX;
+    f.ctas = min(2 * sm_count(dev.device()), kFewCtas);
+    f.min_units = f.snap = 4;
+    f.cuts = reinterpret_cast<PagedCut*>(w);
+    f.part_o = reinterpret_cast<float*>(w + few.o);
+    f.part_ml = reinterpret_cast<float*>(w + few.ml);
+    c.merge_few = cap > (long long)f.snap * kFewKeys;  // else no tile is ever cut
+  }
+  if (c.do_many) {
+    PagedArgs& m = c.many = a;
+    m.rows_min = c.do_few ? kFewRows + 1 : 1;
+    m.rows_max = INT32_MAX;
+    m.ctas = min(sm_count(dev.device()), kManyCtas);
+    m.min_units = m.snap = 2;
+    w += few.bytes;
+    m.cuts = reinterpret_cast<PagedCut*>(w);
+    m.part_o = reinterpret_cast<float*>(w + many.o);
+    m.part_ml = reinterpret_cast<float*>(w + many.ml);
+    c.merge_many = cap > (long long)m.snap * kManyKeys;
+    if (!coded && (paged_map(&c.tk, cache, cache->k) || paged_map(&c.tv, cache, cache->v))) return CN_ERR_CUDA;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return launch_status(who, q->dtype == CN_F16 ? paged_dispatch<__half>(c, cache->dim, coded, dev.device(), s)
+                                               : paged_dispatch<__nv_bfloat16>(c, cache->dim, coded, dev.device(), s));
+}

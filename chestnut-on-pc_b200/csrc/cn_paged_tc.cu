@@ -1,0 +1,754 @@
+// Attention over the paged cache for sequences of many query rows: tcgen05.
+//
+// A tile is 256 query rows (new tokens x the heads of a group) of one sequence
+// and cache head, as two halves of 128 that share every block of 128 keys.
+// S = Q K^T and O += P V both run on tcgen05.mma with M = 128; S, P and O live in
+// tensor memory (columns 0..127 and 128..255: S of the halves, P written over it
+// as 16-bit pairs; 256.. and 384..: O), so the weights never pass through shared
+// memory: P is the A operand of the second product from tensor memory.
+//   warpgroups 0, 1: softmax of a half, one thread a row, the row's 128 scores in
+//                    registers: no shuffles
+//   warpgroup 2:     loads.  A 16-bit cache comes by TMA, a box a page, in the
+//                    128-byte swizzle that the tensor core reads; of an 8-bit one
+//                    the threads hold the codes of the next K and V block in
+//                    registers and store them as f16 (exact) in that swizzle
+//   warp 12:         issues the products: while one half is in its softmax the
+//                    tensor core works for the other one
+// The running maximum is raised only when a block's exceeds it by 2^8 (the sums
+// stay exact, the weights are just up to 256): O is rescaled in tensor memory by
+// the row's own thread then, which is rare after the first blocks.
+// Keys and rows at the edge (tail, causal diagonal, window) are masked in
+// registers.  V rows there that do not exist are zeroed in shared memory, and
+// rows with NaN or infinities, which 0 * inf would carry into rows that do not
+// see them, leave the product and are added by the threads whose row sees them.
+// An 8-bit cache's powers of two: see cn_paged.cu; the loaders leave them as
+// (2^ek * scale, ev, 2^-ev) of each key.
+#include "cn_paged.cuh"
+
+namespace cn {
+
+namespace {
+
+constexpr int kManyRows = 256;
+constexpr int kManyKeys = 128;
+constexpr int kManyThreads = 512;
+constexpr float kLazy = 8.f;  // the maximum may be exceeded by 2^8 before it is raised
+
+// Registers of the warpgroups; the sum is 4 x 128, what the block is launched with.
+template <bool CODED>
+struct ManyRegs {
+  static constexpr int Softmax = CODED ? 176 : 192;
+  static constexpr int Load = CODED ? 96 : 64;
+  static constexpr int Mma = 64;
+  static_assert(2 * Softmax + Load + Mma == 512, "register split");
+};
+
+template <int DIM>
+struct Many {
+  static constexpr int Sub = 128 * 128;            // 128 rows x 64 values of 16 bits
+  static constexpr int Tile = DIM / 64 * Sub;      // 128 rows
+  static constexpr int QBytes = 2 * Tile;
+  static constexpr int Stages = 2;                 // of K, and of V
+  static constexpr size_t Smem = 1024 + QBytes + 2 * Stages * Tile;
+};
+
+struct ManyBars {
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], vfix[2], sfull[2], pfull[2], ofull[2], qfull, qempty;
+  uint32_t tmem;
+};
+
+// The part of a tile that a CTA works on.
+struct ManyPart {
+  int lo;          // position of the tile's unit 0
+  int j0, j1;      // blocks of 128 keys, from lo
+  int a[2], b[2];  // those that the halves take part in
+  int all_lo, all_hi, hi;
+  int rows, row0;
+};
+
+__device__ __forceinline__ ManyPart many_part(const PagedArgs& a, const PagedSeq& q, int tile, int u0, int u1) {
+  ManyPart p;
+  int hi;
+  paged_range<kManyRows, kManyKeys>(a, q, tile, &p.lo, &hi);
+  p.hi = hi;
+  p.row0 = tile * kManyRows;
+  p.rows = min(q.rows - p.row0, kManyRows);
+  p.j0 = u0;
+  p.j1 = min(u1, max((hi - p.lo + kManyKeys - 1) / kManyKeys, u0));
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    p.a[t] = p.b[t] = p.j1;
+    if (p.rows > t * 128 && p.j1 > p.j0) {
+      const int first = q.past + (p.row0 + t * 128) / a.group;
+      const int last = q.past + (min(p.row0 + t * 128 + 128, q.rows) - 1) / a.group;
+      const int thi = last < 0 ? 0 : a.causal ? min(q.len, last + 1) : q.len;
+      const int tlo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+      if (thi > tlo) {
+        p.a[t] = max(p.j0, (tlo - p.lo) / kManyKeys);
+        p.b[t] = min(p.j1, (thi - p.lo + kManyKeys - 1) / kManyKeys);
+        if (p.b[t] < p.a[t]) p.a[t] = p.b[t] = p.j1;
+      }
+    }
+  }
+  const int first_pos = q.past + p.row0 / a.group, last_pos = q.past + (p.row0 + p.rows - 1) / a.group;
+  p.all_hi = first_pos < 0 ? 0 : a.causal ? min(q.len, first_pos + 1) : q.len;
+  p.all_lo = a.window > 0 ? last_pos - a.window + 1 : 0;
+  return p;
+}
+
+// Whether some row of the tile does not see all of block j.
+__device__ __forceinline__ bool many_edge(const ManyPart& p, int j) {
+  const int k0 = p.lo + j * kManyKeys;
+  return k0 < p.all_lo || k0 + kManyKeys > p.all_hi;
+}
+
+// A warp's wait: the same answer for all its lanes.
+__device__ __forceinline__ bool many_wait(uint64_t* bar, uint32_t parity, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,"
+      "%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  return r;
+}
+
+// D[tmem] += A[tmem] * B[smem], 16-bit operands.
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.eq.u32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc)
+      : "memory");
+}
+
+template <typename M>
+__device__ __forceinline__ constexpr uint32_t many_idesc(int n, bool b_mn_major) {
+  constexpr uint32_t f = std::is_same_v<M, __nv_bfloat16> ? 1u : 0u;  // operand format, both alike
+  return umma_idesc_f16(n, b_mn_major) | (f << 7) | (f << 10);
+}
+
+template <typename M>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same_v<M, __nv_bfloat16> ? 0x7f80u : 0x7c00u;
+  return (w & e) == e || (w & (e << 16)) == (e << 16);
+}
+
+__device__ __forceinline__ void load_group_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+// T: q and out (and a 16-bit cache).
+template <typename T, int DIM, bool CODED>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    k_paged_many(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
+  using L = Many<DIM>;
+  using M = std::conditional_t<CODED, __half, T>;
+  using R = ManyRegs<CODED>;
+  extern __shared__ uint8_t many_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sq = smem;
+  uint8_t* sk = smem + L::QBytes;
+  uint8_t* sv = sk + L::Stages * L::Tile;
+  __shared__ PagedScratch<kManyThreads> sc;
+  __shared__ ManyBars bar;
+  __shared__ uint32_t bad[2][4];                        // V rows of an edge block that are not finite
+  __shared__ __align__(16) float kx[CODED ? 2 : 1][CODED ? 128 : 1][2];  // (scale 2^ek, -) of a K block
+  __shared__ __align__(16) float vx[CODED ? 2 : 1][CODED ? 128 : 1][2];  // (ev, 2^-ev) of a V block
+  __shared__ float qpow[2][CODED ? kManyRows : 1];      // power of two that a row of Q was divided by (parts in turn)
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.kfull[i], CODED ? 128 : 1);
+      mbar_init(&bar.vfull[i], CODED ? 128 : 1);
+      mbar_init(&bar.kempty[i], 1);
+      mbar_init(&bar.vempty[i], 1);
+      mbar_init(&bar.vfix[i], 128);
+      mbar_init(&bar.sfull[i], 1);
+      mbar_init(&bar.pfull[i], 128);
+      mbar_init(&bar.ofull[i], 1);
+    }
+    mbar_init(&bar.qfull, 128);
+    mbar_init(&bar.qempty, 1);
+    fence_barrier_init();
+    if constexpr (!CODED) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+  }
+  if (warp == 13) {
+    tmem_alloc(&bar.tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  pdl_trigger();
+  pdl_wait();
+  paged_find<kManyRows, kManyKeys, kManyThreads>(a, blockIdx.x, &sc);
+  if (tid == 0) a.cuts[blockIdx.x] = sc.cut[0];
+  long long at = sc.cut[0].start;
+  const long long end = sc.cut[1].start;
+  int s = sc.cut[0].seq, head = sc.cut[0].head, tile = sc.cut[0].tile;
+  long long first = sc.cut[0].first;
+  PagedSeq q = {};
+  bool more = at < end;
+  if (more) q = paged_seq<kManyRows>(a, s);
+  // Every role walks the same parts: advance() steps to the next one.
+  int units = 0, u0 = 0, u1 = 0;
+  auto part = [&]() {
+    units = paged_units<kManyRows, kManyKeys>(a, q, tile);
+    u0 = (int)(at - first);
+    u1 = (int)min((long long)units, end - first);
+    return many_part(a, q, tile, u0, u1);
+  };
+  auto advance = [&]() {
+    at = first + u1;
+    first += units;
+    more = at < end && paged_next<kManyRows>(a, &q, &s, &head, &tile);
+  };
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::Softmax));
+    const int t = warp >> 2, r = tid & 127;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
+    uint32_t ns = 0, no = 0, nb = 0, np = 0, fixes = 0;  // S blocks, O tiles, blocks and parts so far; fixes: phase bit of a stage
+    bool ok = true;
+    for (; more && ok; advance()) {
+      const ManyPart p = part();
+      const int row = p.row0 + t * 128 + r;
+      const bool live = t * 128 + r < p.rows;
+      const int pos = live ? q.past + row / a.group : -1;
+      const int see_hi = pos < 0 ? 0 : a.causal ? min(q.len, pos + 1) : q.len;
+      const int see_lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
+      float m = -INFINITY, l = 0.f;
+      const int ja = p.a[t], jb = p.b[t];
+      if (ja < jb) {
+        uint32_t z[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) z[i] = 0u;
+#pragma unroll
+        for (int c = 0; c < DIM; c += 32) tmem_st32(to + c, z);
+        tmem_st_wait();
+      }
+      float rs = 1.f;
+      for (int j = p.j0; j < p.j1 && ok; ++j) {
+        const uint32_t st = (nb + j - p.j0) & 1;
+        const bool edge = many_edge(p, j);
+        const uint32_t fix = (fixes >> st) & 1;
+        if (edge) fixes ^= 1u << st;
+        if (j < ja || j >= jb) continue;
+        ok = many_wait(&bar.sfull[t], ns & 1, 3);
+        if (!ok) break;
+        ++ns;
+        tc_fence_after();
+        if constexpr (CODED && std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][t * 128 + r];
+        const int k0 = p.lo + j * kManyKeys;
+        uint32_t raw[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32(ts + c, raw + c);
+        if (edge) {  // its V is in order, and what lies beside it
+          ok = many_wait(&bar.vfix[st], fix, 2);
+          if (!ok) break;
+        }
+        if constexpr (CODED) {
+          ok = many_wait(&bar.vfull[st], ((nb + j - p.j0) >> 1) & 1, 1);
+          if (!ok) break;
+        }
+        tmem_ld_wait();
+        float x[128];
+#pragma unroll
+        for (int c = 0; c < 128; ++c) x[c] = __uint_as_float(raw[c]);
+        if constexpr (CODED) {
+#pragma unroll
+          for (int c = 0; c < 128; c += 2) {
+            const float4 ke = *reinterpret_cast<const float4*>(kx[st][c]);
+            const float4 ve = *reinterpret_cast<const float4*>(vx[st][c]);
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+              x[c] *= rs;
+              x[c + 1] *= rs;
+            }
+            x[c] = fmaf(x[c], ke.x, ve.x);
+            x[c + 1] = fmaf(x[c + 1], ke.z, ve.z);
+          }
+        }
+        if (edge) {
+          const int clo = see_lo - k0, chi = see_hi - k0;
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (c < clo || c >= chi) x[c] = -INFINITY;
+        }
+        float mx[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = x[i];
+#pragma unroll
+        for (int c = 4; c < 128; c += 4)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], x[c + i]);
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if constexpr (!CODED) top *= a.scale;
+        const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+        if (__any_sync(0xffffffffu, raise)) {
+          // S of this block was complete after every product before it: O stands still
+          const float c = raise ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
+          if (raise) m = top;
+          l *= c;
+          if (j > ja) {
+#pragma unroll
+            for (int d = 0; d < DIM; d += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + d, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+              tmem_st32(to + d, o);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.f : -m;
+        if (edge) {
+          // rows of V that are not finite: for the rows that see them, from the cache itself
+#pragma unroll 1
+          for (int w = 0; w < 4; ++w) {
+            uint32_t bits = bad[st][w];
+#pragma unroll 1
+            while (bits) {
+              const int c = w * 32 + __ffs(bits) - 1;
+              bits &= bits - 1;
+              float sx = __uint_as_float(tmem_ld1(ts + c));
+              tmem_ld_wait();
+              if constexpr (CODED)
+                sx = exp2_approx(fmaf(sx * rs, kx[st][c][0], vx[st][c][0]) + sub);
+              else
+                sx = exp2_approx(fmaf(sx, a.scale, sub));
+              const int key = k0 + c;
+              const bool see = key >= see_lo && key < see_hi;
+              const int page = page_of(a.b, s, key);
+              const long long vr = (((long long)max(page, 0) * a.heads + head) << a.b.page_shift) + (key & ((1 << a.b.page_shift) - 1));
+#pragma unroll 1
+              for (int d = 0; d < DIM; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(to + d, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                  float2 v;
+                  if constexpr (CODED)
+                    v = Num<__half>::unpack(codes_to_h2(*reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(a.v) + vr * DIM + d + i)));
+                  else
+                    v = Num<T>::unpack(*reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v) + vr * DIM + d + i));
+                  if (see) {
+                    o[i] = __float_as_uint(fmaf(sx, v.x, __uint_as_float(o[i])));
+                    o[i + 1] = __float_as_uint(fmaf(sx, v.y, __uint_as_float(o[i + 1])));
+                  }
+                }
+                tmem_st32(to + d, o);
+              }
+              tmem_st_wait();
+            }
+          }
+        }
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 128; h += 64) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int c = h; c < h + 64; c += 4) {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = exp2_approx(CODED ? x[c + i] + sub : fmaf(x[c + i], a.scale, sub));
+            if constexpr (CODED) {
+              const float4 v0 = *reinterpret_cast<const float4*>(vx[st][c]);
+              const float4 v1 = *reinterpret_cast<const float4*>(vx[st][c + 2]);
+              sum[0] = fmaf(e[0], v0.y, sum[0]);
+              sum[1] = fmaf(e[1], v0.w, sum[1]);
+              sum[2] = fmaf(e[2], v1.y, sum[2]);
+              sum[3] = fmaf(e[3], v1.w, sum[3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sum[i] += e[i];
+            }
+            pk[(c - h) / 2] = Num<M>::pack(e[0], e[1]);
+            pk[(c - h) / 2 + 1] = Num<M>::pack(e[2], e[3]);
+          }
+          tmem_st32(ts + h / 2, pk);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bar.pfull[t]);
+      }
+      nb += p.j1 - p.j0;
+      np += p.j1 > p.j0;
+      if (!ok) break;
+      // ---- out, or this part's sums
+      const bool complete = u0 == 0 && u1 == units;
+      const long long slot = 2ll * blockIdx.x + (u0 == 0 ? 1 : 0);
+      if (ja < jb) {
+        ok = many_wait(&bar.ofull[t], no & 1, 3);
+        ++no;
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const float inv = m == -INFINITY ? 0.f : 1.f / l;
+      T* out = static_cast<T*>(a.out) + (long long)(q.tok0 + row / a.group) * a.o_token +
+               (long long)(head * a.group + row % a.group) * a.o_head;
+      const long long pr = slot * kManyRows + t * 128 + r;
+#pragma unroll
+      for (int d = 0; d < DIM; d += 32) {
+        uint32_t o[32];
+        if (ja < jb) {
+          tmem_ld32(to + d, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (live) {
+          if (complete) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = Num<T>::pack(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4*>(out + d + i) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(a.part_o + pr * DIM + d + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
+        }
+      }
+      if (live && !complete) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(m, l);
+      tc_fence_before();  // the next part's zeros and products come after these loads
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------ loads
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Load));
+    const int lt = tid - 256;
+    uint32_t nb = 0, np = 0;  // blocks, parts with blocks so far
+    bool ok = true;
+    const int shift = a.b.page_shift, page_rows = 1 << shift;
+    const int box_rows = min(page_rows, kManyKeys);
+    for (; more && ok; advance()) {
+      const ManyPart p = part();
+      if (p.j0 >= p.j1) continue;
+      const int blocks = p.j1 - p.j0;
+
+      // 16-bit cache: thread 0 asks for block j of K or V
+      auto fetch = [&](int j, uint32_t n, const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty) {
+        const uint32_t st = n & 1;
+        if (n >= 2 && !mbar_wait(&empty[st], ((n >> 1) & 1) ^ 1, 2)) return false;
+        const int k0 = p.lo + j * kManyKeys;
+        const int boxes = (min(kManyKeys, p.hi - k0) + box_rows - 1) / box_rows;
+        uint32_t bytes = 0;
+        for (int i = 0; i < boxes; ++i) bytes += page_of(a.b, s, k0 + i * box_rows) >= 0 ? box_rows * DIM * 2 : 0;
+        mbar_arrive_expect_tx(&full[st], bytes);
+        for (int i = 0; i < boxes; ++i) {
+          const int page = page_of(a.b, s, k0 + i * box_rows);
+          if (page < 0) continue;
+          const int y = head * page_rows + ((k0 + i * box_rows) & (page_rows - 1));
+#pragma unroll
+          for (int d = 0; d < DIM / 64; ++d)
+            tma_load_3d(ring + st * L::Tile + d * L::Sub + i * box_rows * 128, map, &full[st], d * 64, y, page);
+        }
+        return true;
+      };
+      // 8-bit cache: a thread's codes of block j, 16 a piece; piece lt + 128 i
+      constexpr int PR = DIM / 16;                 // pieces of a row
+      constexpr int PT = CODED ? 128 * PR / 128 : 1;  // pieces of a thread
+      auto hold = [&](int j, const void* cache, uint4 (&c)[PT]) {
+        const int k0 = p.lo + j * kManyKeys;
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+          const int key = k0 + (lt + 128 * i) / PR;
+          c[i] = make_uint4(0, 0, 0, 0);
+          if (key < p.hi) {
+            const int page = page_of(a.b, s, key);
+            if (page >= 0) {
+              const long long kr = (((long long)page * a.heads + head) << shift) + (key & (page_rows - 1));
+              c[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + kr * DIM + ((lt + 128 * i) % PR) * 16);
+            }
+          }
+        }
+      };
+      auto hold_exp = [&](int j, const uint8_t* exps) -> uint32_t {
+        const int key = p.lo + j * kManyKeys + lt;
+        if (key >= p.hi) return 127u;
+        const int page = page_of(a.b, s, key);
+        return page < 0 ? 127u : exps[(((long long)page * a.heads + head) << shift) + (key & (page_rows - 1))];
+      };
+      auto put = [&](const uint4 (&c)[PT], uint8_t* to) {
+#pragma unroll
+        for (int i = 0; i < PT; ++i) {
+          const int row = (lt + 128 * i) / PR, piece = (lt + 128 * i) % PR;
+          const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+          uint32_t h[8];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            h[2 * e] = codes_to_h2(w[e] & 0xffffu);
+            h[2 * e + 1] = codes_to_h2(w[e] >> 16);
+          }
+          uint8_t* base = to + (piece >> 2) * L::Sub + row * 128;
+          const int ch = (piece & 3) * 2;
+          *reinterpret_cast<uint4*>(base + ((ch ^ (row & 7)) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(base + (((ch + 1) ^ (row & 7)) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+      };
+
+      uint4 ck[PT], cv[PT];
+      uint32_t ek = 0, ev = 0;
+      if constexpr (CODED) {
+        hold(p.j0, a.k, ck);
+        ek = hold_exp(p.j0, a.k_exp);
+        hold(p.j0, a.v, cv);
+        ev = hold_exp(p.j0, a.v_exp);
+      } else {
+        if (lt == 0) ok = fetch(p.j0, nb, &tm_k, sk, bar.kfull, bar.kempty);
+        ok = __all_sync(0xffffffffu, ok);
+      }
+
+      // ---- Q: 128 or 256 rows, swizzled
+      if (np > 0 && ok) ok = many_wait(&bar.qempty, (np - 1) & 1, 2);
+      ++np;
+      const int qrows = p.rows > 128 ? 256 : 128;
+      constexpr int CH = DIM / 8;  // 16-byte pieces of a row
+      auto q_src = [&](int i) {
+        const int row = p.row0 + min(i / CH, p.rows - 1);
+        return static_cast<const T*>(a.q) + (long long)(q.tok0 + row / a.group) * a.q_token +
+               (long long)(head * a.group + row % a.group) * a.q_head + (i % CH) * 8;
+      };
+      auto q_dst = [&](int i) {
+        const int r = i / CH, ch = i % CH;
+        return sq + (r >> 7) * L::Tile + (ch >> 3) * L::Sub + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) * 16);
+      };
+      if constexpr (CODED && std::is_same_v<T, __nv_bfloat16>) {
+        // to f16 by the row's power of two (see cn_paged.cu); CH lanes hold a row
+#pragma unroll 1
+        for (int i0 = lt; i0 < qrows * CH; i0 += 128 * 4) {
+          uint4 w[4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            w[x] = (i0 + x * 128) / CH < p.rows ? *reinterpret_cast<const uint4*>(q_src(i0 + x * 128)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int i = i0 + x * 128;
+            uint32_t v[4] = {w[x].x, w[x].y, w[x].z, w[x].w};
+            float mx = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = Num<T>::unpack(v[e]);
+              mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+#pragma unroll
+            for (int o = CH / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const uint32_t eb = min(max(__float_as_uint(mx) >> 23, 16u), 238u);
+            const float by = __uint_as_float((254u + 13u - eb) << 23);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = Num<T>::unpack(v[e]);
+              v[e] = Num<__half>::pack(f.x * by, f.y * by);
+            }
+            *reinterpret_cast<uint4*>(q_dst(i)) = make_uint4(v[0], v[1], v[2], v[3]);
+            if (i % CH == 0) qpow[(np - 1) & 1][i / CH] = __uint_as_float((eb - 13u) << 23);
+          }
+        }
+      } else {
+#pragma unroll 4
+        for (int i = lt; i < qrows * CH; i += 128) cp_async16_or_zero(smem_u32(q_dst(i)), q_src(i), i / CH < p.rows);
+        cp_async_wait_all();
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&bar.qfull);
+
+      // ---- blocks
+      for (int i = 0; i < blocks && ok; ++i) {
+        const int j = p.j0 + i;
+        const uint32_t n = nb + i, st = n & 1;
+        const bool edge = many_edge(p, j);
+        if constexpr (CODED) {
+          if (n >= 2) ok = many_wait(&bar.kempty[st], ((n >> 1) & 1) ^ 1, 2);
+          if (!ok) break;
+          // kx and vx of a stage are read by the softmax of its block, which is over when its
+          // products with V are: kempty alone would not say so
+          if (n >= 2) ok = many_wait(&bar.vempty[st], ((n >> 1) & 1) ^ 1, 2);
+          if (!ok) break;
+          put(ck, sk + st * L::Tile);
+          kx[st][lt][0] = exp_byte(ek) * a.scale;
+          fence_proxy_async_smem();
+          mbar_arrive(&bar.kfull[st]);
+          if (i + 1 < blocks) {
+            hold(j + 1, a.k, ck);
+            ek = hold_exp(j + 1, a.k_exp);
+          }
+          put(cv, sv + st * L::Tile);
+          vx[st][lt][0] = (float)((int)ev - 127);
+          vx[st][lt][1] = exp_byte(254u - ev);
+          fence_proxy_async_smem();
+          mbar_arrive(&bar.vfull[st]);
+          if (i + 1 < blocks) {
+            hold(j + 1, a.v, cv);
+            ev = hold_exp(j + 1, a.v_exp);
+          }
+        } else {
+          if (lt == 0) {
+            ok = fetch(j, n, &tm_v, sv, bar.vfull, bar.vempty);
+            if (ok && i + 1 < blocks) ok = fetch(j + 1, n + 1, &tm_k, sk, bar.kfull, bar.kempty);
+          }
+          ok = __all_sync(0xffffffffu, ok);
+        }
+        if (edge && ok) {
+          ok = many_wait(&bar.vfull[st], (n >> 1) & 1, 1);
+          const int key = p.lo + j * kManyKeys + lt;
+          uint8_t* vr = sv + st * L::Tile + lt * 128;
+          bool odd = false;
+          if (key < q.len && key < p.hi) {
+#pragma unroll
+            for (int d = 0; d < DIM / 64; ++d)
+#pragma unroll 4
+              for (int c = 0; c < 8; ++c) {
+                const uint4 w = *reinterpret_cast<const uint4*>(vr + d * L::Sub + ((c + lt) & 7) * 16);
+                odd |= not_finite2<M>(w.x) | not_finite2<M>(w.y) | not_finite2<M>(w.z) | not_finite2<M>(w.w);
+              }
+          }
+          if (odd || key >= q.len || key >= p.hi) {
+#pragma unroll
+            for (int d = 0; d < DIM / 64; ++d)
+#pragma unroll 4
+              for (int c = 0; c < 8; ++c)
+                *reinterpret_cast<uint4*>(vr + d * L::Sub + ((c + lt) & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          const uint32_t bits = __ballot_sync(0xffffffffu, odd);
+          if (lane == 0) bad[st][warp - 8] = bits;
+          fence_proxy_async_smem();
+          mbar_arrive(&bar.vfix[st]);
+        }
+      }
+      nb += blocks;
+    }
+    if (!ok && !CODED && lt == 0) {  // given up: the copies in flight land before the block ends
+      const unsigned long long t0 = global_ns();
+      while (global_ns() - t0 < 100000000ull) {
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Mma));
+    if (warp == 12 && lane == 0) {
+      // ------------------------------------------------------------ products
+      constexpr uint32_t id_s = many_idesc<M>(kManyKeys, false), id_o = many_idesc<M>(DIM, true);
+      uint32_t nb = 0, np = 0, ns[2] = {0, 0}, fixes = 0;
+      bool ok = true;
+      auto scores = [&](int t, uint32_t st) {
+        const uint32_t qa = smem_u32(sq) + t * L::Tile, ka = smem_u32(sk) + st * L::Tile;
+#pragma unroll
+        for (int k = 0; k < DIM / 16; ++k) {
+          const uint32_t off = (k >> 2) * L::Sub + (k & 3) * 32;
+          tc_mma_f16(tmem + t * 128, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024), id_s, k > 0);
+        }
+        tc_commit(&bar.sfull[t]);
+      };
+      for (; more && ok; advance()) {
+        const ManyPart p = part();
+        if (p.j0 >= p.j1) continue;
+        ok = mbar_wait(&bar.qfull, np & 1, 1) && mbar_wait(&bar.kfull[nb & 1], (nb >> 1) & 1, 1);
+        if (!ok) break;
+        ++np;
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (p.a[t] == p.j0 && p.a[t] < p.b[t]) scores(t, nb & 1);
+        tc_commit(&bar.kempty[nb & 1]);
+        if (p.j1 == p.j0 + 1) tc_commit(&bar.qempty);
+        for (int j = p.j0; j < p.j1 && ok; ++j) {
+          const uint32_t n = nb + j - p.j0, st = n & 1;
+          bool v_there = false, k_there = false;
+          auto need_v = [&]() {
+            if (v_there) return true;
+            v_there = true;
+            bool good = mbar_wait(&bar.vfull[st], (n >> 1) & 1, 1);
+            if (good && many_edge(p, j)) good = mbar_wait(&bar.vfix[st], (fixes >> st) & 1, 1);
+            return good;
+          };
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >= p.a[t] && j < p.b[t]) {
+              ok = ok && need_v() && mbar_wait(&bar.pfull[t], ns[t] & 1, 3);
+              if (!ok) break;
+              ++ns[t];
+              tc_fence_after();
+              const uint32_t va = smem_u32(sv) + st * L::Tile;
+#pragma unroll
+              for (int k = 0; k < kManyKeys / 16; ++k)
+                tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, umma_desc_sw128(va + k * 2048, L::Sub, 1024), id_o);
+              if (j + 1 == p.b[t]) tc_commit(&bar.ofull[t]);
+            }
+            if (j + 1 >= p.a[t] && j + 1 < p.b[t]) {
+              if (!k_there) {
+                k_there = true;
+                ok = ok && mbar_wait(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, 1);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              scores(t, (n + 1) & 1);
+            }
+          }
+          if (!ok) break;
+          if (!v_there) ok = need_v();  // a block that neither half sees: its loads end before its stage is free
+          if (j + 1 < p.j1) {
+            if (!k_there) ok = ok && mbar_wait(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, 1);
+            tc_commit(&bar.kempty[(n + 1) & 1]);
+            if (j + 2 == p.j1) tc_commit(&bar.qempty);
+          }
+          tc_commit(&bar.vempty[st]);
+          if (many_edge(p, j)) fixes ^= 1u << st;
+        }
+        nb += p.j1 - p.j0;
+      }
+      // the last products' arrivals land before the block ends
+      if (ok && np > 0) {
+        mbar_wait(&bar.kempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
+        mbar_wait(&bar.qempty, (np - 1) & 1, 3);
+        mbar_wait(&bar.vempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
+      }
+    }
+    __syncwarp();
+  }
+  // Every product's result was waited for by the softmax that used it; the others (a give-up) end here.
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 13) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+}  // namespace cn

@@ -311,7 +311,7 @@ int cn_kv_read(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_head
  * nothing is zeros, and what is not visible has no influence, whatever its value.
  * Query head h reads cache head h / (q.heads / cache.heads).  q and out alike in
  * dtype (CN_F16 or CN_BF16, the cache's own unless that is CN_E4M3), heads and
- * dim; out may be q.  Statistics and sums in f32, the weights enter the product
+ * dim; out may be q; scale positive and finite.  Statistics and sums in f32, the weights enter the product
  * with V in 16 bits.  workspace: cn_paged_attention_workspace() bytes, 256-byte
  * aligned, its content of no matter before and after a call; calls that may run
  * at the same time need one each.  Results do not depend on timing. */
