@@ -100,29 +100,31 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
   const int g = lane >> 2, t4 = lane & 3;
   pdl_trigger();
   pdl_wait();
-  paged_find<kFewRows, kFewKeys, kFewThreads>(a, blockIdx.x, &sc);
+  paged_find<kFewKeys, kFewThreads>(a, blockIdx.x, &sc);
   long long at = sc.cut[0].start;
   const long long end = sc.cut[1].start;
   if (tid == 0) a.cuts[blockIdx.x] = sc.cut[0];
   if (at >= end) return;
   int s = sc.cut[0].seq, head = sc.cut[0].head, b = sc.cut[0].tile;
   long long first = sc.cut[0].first;
-  PagedSeq sq = paged_seq<kFewRows>(a, s);
+  PagedSeq sq = paged_seq(a, s);
   uint8_t* ring = few_smem + warp * F::Warp;
   const uint32_t ring_u = smem_u32(ring);
   const int page_rows = 1 << a.b.page_shift;
 
   while (true) {
-    const int units = paged_units<kFewRows, kFewKeys>(a, sq, b);
+    const int units = paged_units<kFewKeys>(a, sq, b);
     int lo, hi;
-    paged_range<kFewRows, kFewKeys>(a, sq, b, &lo, &hi);
+    const int tok0 = b * a.tile_tokens, toks = paged_tokens(a, sq, b);
+    paged_range<kFewKeys>(a, sq, tok0, toks, &lo, &hi);
     const int u0 = (int)(at - first), u1 = (int)min((long long)units, end - first);
-    const int row0 = b * kFewRows, rows = min(sq.rows - row0, kFewRows);
+    const int rows = toks * a.group;
+    auto token_of = [&](int r) { return div_by(r, a.group, a.group_mul); };
     // positions of this thread's rows g and g + 8; none: -1 sees nothing
-    const int pos_a = g < rows ? sq.past + (row0 + g) / a.group : -1;
-    const int pos_b = g + 8 < rows ? sq.past + (row0 + g + 8) / a.group : -1;
+    const int pos_a = g < rows ? sq.past + tok0 + token_of(g) : -1;
+    const int pos_b = g + 8 < rows ? sq.past + tok0 + token_of(g + 8) : -1;
     // every row of the tile sees the keys [all_lo, all_hi)
-    const int first_pos = sq.past + row0 / a.group, last_pos = sq.past + (row0 + rows - 1) / a.group;
+    const int first_pos = sq.past + tok0, last_pos = first_pos + toks - 1;
     const int all_hi = first_pos < 0 ? 0 : a.causal ? min(sq.len, first_pos + 1) : sq.len;
     const int all_lo = a.window > 0 ? last_pos - a.window + 1 : 0;
 
@@ -130,11 +132,12 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
     uint32_t qf[KS][4];
     float rs_a = a.scale, rs_b = a.scale;  // powers of two (of log2 e / scale) that a product stands for
     {
-      const int ra = row0 + min(g, rows - 1), rb = row0 + min(g + 8, rows - 1);
-      const T* qa = static_cast<const T*>(a.q) + (long long)(sq.tok0 + ra / a.group) * a.q_token +
-                    (long long)(head * a.group + ra % a.group) * a.q_head;
-      const T* qb = static_cast<const T*>(a.q) + (long long)(sq.tok0 + rb / a.group) * a.q_token +
-                    (long long)(head * a.group + rb % a.group) * a.q_head;
+      const int ra = min(g, rows - 1), rb = min(g + 8, rows - 1);
+      const int ta = token_of(ra), tb = token_of(rb);
+      const T* qa = static_cast<const T*>(a.q) + (long long)(sq.tok0 + tok0 + ta) * a.q_token +
+                    (long long)(head * a.group + ra - ta * a.group) * a.q_head;
+      const T* qb = static_cast<const T*>(a.q) + (long long)(sq.tok0 + tok0 + tb) * a.q_token +
+                    (long long)(head * a.group + rb - tb * a.group) * a.q_head;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         // value index of the k pair (lo: 2 t4, hi: 2 t4 + 8); coded: the order of the codes' pieces
@@ -457,9 +460,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
       }
       if (complete) {
         const float inv = m == -INFINITY ? 0.f : 1.f / l;
-        const int row = row0 + r;
-        T* out = static_cast<T*>(a.out) + (long long)(sq.tok0 + row / a.group) * a.o_token +
-                 (long long)(head * a.group + row % a.group) * a.o_head + d;
+        const int i = token_of(r);
+        T* out = static_cast<T*>(a.out) + (long long)(sq.tok0 + tok0 + i) * a.o_token +
+                 (long long)(head * a.group + r - i * a.group) * a.o_head + d;
         *reinterpret_cast<uint2*>(out) = make_uint2(Num<T>::pack(sum.x * inv, sum.y * inv), Num<T>::pack(sum.z * inv, sum.w * inv));
       } else {
         *reinterpret_cast<float4*>(a.part_o + (slot * kFewRows + r) * DIM + d) = sum;
@@ -469,7 +472,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
     at = first + u1;
     if (at >= end) break;
     first += units;
-    if (!paged_next<kFewRows>(a, &sq, &s, &head, &b)) break;
+    if (!paged_next(a, &sq, &s, &head, &b)) break;
     __syncthreads();  // the join's memory becomes rings again
   }
 }
@@ -486,9 +489,13 @@ __global__ void __launch_bounds__(RPB * 32) k_paged_merge(const PagedArgs a) {
   const int c = blockIdx.x + 1;
   const PagedCut cut = a.cuts[c];
   if (cut.start >= cut.total || cut.start <= cut.first || a.cuts[c - 1].start > cut.first) return;
-  const PagedSeq sq = paged_seq<ROWS>(a, cut.seq);
+  const PagedSeq sq = paged_seq(a, cut.seq);
   const int r = blockIdx.y * RPB + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (cut.tile * ROWS + r >= sq.rows) return;
+  // row r: of half r / HALF, there token i, query head h of the group
+  constexpr int HALF = ROWS == 256 ? 128 : ROWS;
+  const int in_half = r % HALF, i0 = div_by(in_half, a.group, a.group_mul);
+  const int i = r / HALF * a.half_tokens + i0, h = in_half - i0 * a.group;
+  if (i0 >= a.half_tokens || i >= paged_tokens(a, sq, cut.tile)) return;
   int last = c;  // the last CTA with a part
   while (last + 1 < a.ctas && a.cuts[last + 1].start < cut.first + cut.units) ++last;
   constexpr int V = DIM / 32;
@@ -509,9 +516,8 @@ __global__ void __launch_bounds__(RPB * 32) k_paged_merge(const PagedArgs a) {
     for (int x = 0; x < V; ++x) o[x] = o[x] * co + f[x] * cp;
   }
   const float inv = m == -INFINITY ? 0.f : 1.f / l;
-  const int row = cut.tile * ROWS + r;
-  T* out = static_cast<T*>(a.out) + (long long)(sq.tok0 + row / a.group) * a.o_token +
-           (long long)(cut.head * a.group + row % a.group) * a.o_head;
+  T* out = static_cast<T*>(a.out) + (long long)(sq.tok0 + cut.tile * a.tile_tokens + i) * a.o_token +
+           (long long)(cut.head * a.group + h) * a.o_head;
 #pragma unroll
   for (int x = 0; x < V; ++x) {
     const uint32_t w = Num<T>::pack(o[x] * inv, 0.f);

@@ -1,8 +1,9 @@
 // How the attention over a paged cache is cut into work, shared by its kernels.
 //
-// A tile is up to ROWS query rows that read the same keys: rows of one sequence
-// and one cache head, row r = (new token r / group, query head r % group of the
-// group).  Its keys are cut into units of KEYS positions.  All units of all
+// A tile is the query rows of up to tile_tokens new tokens of a sequence that
+// read one cache head: token i's query head g of the group is row i * group + g
+// (of the half that the token lies in, where the kernel has two of 128 rows).
+// Its keys are cut into units of KEYS positions.  All units of all
 // tiles, in the order (sequence, cache head, tile, unit), are one line, and CTA
 // c of W takes the c-th equal stretch of it: sequences of any mix of lengths
 // keep every SM busy to the end, and one long context is spread over all of
@@ -26,6 +27,8 @@ struct PagedArgs {
   const void *k, *v;
   const uint8_t *k_exp, *v_exp;
   int heads, group;     // cache heads, query heads of each
+  uint32_t group_mul;   // divides rows by group: see div_by
+  int tile_tokens, half_tokens;
   float scale;          // the caller's scale * log2(e)
   int causal, window;
   int rows_min, rows_max;  // this launch takes the sequences with rows in [rows_min, rows_max]
@@ -43,10 +46,15 @@ struct PagedCut {
 };
 
 struct PagedSeq {
-  int tok0, n, len, past, rows, tiles;
+  int tok0, n, len, past, tiles;
 };
 
-template <int ROWS>
+// n / d for mul = min(2^32 / d, 2^32 - 1): the product is the quotient or one less.
+__device__ __forceinline__ int div_by(int n, int d, uint32_t mul) {
+  const int q = (int)__umulhi((uint32_t)n, mul);
+  return n - q * d >= d ? q + 1 : q;
+}
+
 __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int s) {
   PagedSeq q;
   const long long t0 = min((long long)max(a.b.cu[s], 0), a.b.tokens);
@@ -57,26 +65,29 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int s) {
   q.past = len - q.n;
   q.len = min(len, a.b.table_width << a.b.page_shift);
   if (q.len < len && q.n > 0) set_dev_error(kErrPage);
-  q.rows = q.n * a.group;
-  if (q.rows < a.rows_min || q.rows > a.rows_max) q.rows = 0;
-  q.tiles = (q.rows + ROWS - 1) / ROWS;
+  const int rows = q.n * a.group;
+  q.tiles = rows < a.rows_min || rows > a.rows_max ? 0 : (q.n + a.tile_tokens - 1) / a.tile_tokens;
   return q;
 }
 
-// Keys [lo, hi) that any row of tile b sees, lo rounded down to a unit.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedSeq& q, int b, int* lo, int* hi) {
-  const int first = q.past + b * ROWS / a.group;                                // position of the first row
-  const int last = q.past + (min((b + 1) * ROWS, q.rows) - 1) / a.group;        // and of the last one
+// Tokens of tile b.
+__device__ __forceinline__ int paged_tokens(const PagedArgs& a, const PagedSeq& q, int b) {
+  return min(q.n - b * a.tile_tokens, a.tile_tokens);
+}
+
+// Keys [lo, hi) that tokens [t0, t0 + n) see, lo rounded down to a unit.
+template <int KEYS>
+__device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedSeq& q, int t0, int n, int* lo, int* hi) {
+  const int first = q.past + t0, last = first + n - 1;  // positions
   *hi = last < 0 ? 0 : a.causal ? min(q.len, last + 1) : q.len;
   *lo = a.window > 0 ? max(first - a.window + 1, 0) / KEYS * KEYS : 0;
 }
 
 // Units of tile b: at least one, so that rows without keys are written too.
-template <int ROWS, int KEYS>
+template <int KEYS>
 __device__ __forceinline__ int paged_units(const PagedArgs& a, const PagedSeq& q, int b) {
   int lo, hi;
-  paged_range<ROWS, KEYS>(a, q, b, &lo, &hi);
+  paged_range<KEYS>(a, q, b * a.tile_tokens, paged_tokens(a, q, b), &lo, &hi);
   return max((hi - lo + KEYS - 1) / KEYS, 1);
 }
 
@@ -114,24 +125,24 @@ struct PagedScratch {
 
 // Units of one head of sequences s0 .. s0 + THREADS - 1 into sc->seq_units.  A
 // warp takes a sequence and its lanes the tiles, a thread where a sequence has
-// one tile at most (ROWS >= rows_max).
-template <int ROWS, int KEYS, int THREADS>
+// one tile at most.
+template <int KEYS, int THREADS>
 __device__ __forceinline__ void paged_count(const PagedArgs& a, int s0, PagedScratch<THREADS>* sc) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int n = min(a.b.n_seqs - s0, THREADS);
-  if (a.rows_max <= ROWS) {
+  if (a.rows_max <= a.tile_tokens * a.group) {
     int w = 0;
     if (tid < n) {
-      const PagedSeq q = paged_seq<ROWS>(a, s0 + tid);
-      if (q.tiles) w = paged_units<ROWS, KEYS>(a, q, 0);
+      const PagedSeq q = paged_seq(a, s0 + tid);
+      if (q.tiles) w = paged_units<KEYS>(a, q, 0);
     }
     sc->seq_units[tid] = w;
   } else {
     for (int i = tid >> 5; i < THREADS; i += THREADS / 32) {
       int w = 0;
       if (i < n) {
-        const PagedSeq q = paged_seq<ROWS>(a, s0 + i);
-        for (int b = lane; b < q.tiles; b += 32) w += paged_units<ROWS, KEYS>(a, q, b);
+        const PagedSeq q = paged_seq(a, s0 + i);
+        for (int b = lane; b < q.tiles; b += 32) w += paged_units<KEYS>(a, q, b);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
       }
@@ -143,13 +154,13 @@ __device__ __forceinline__ void paged_count(const PagedArgs& a, int s0, PagedScr
 
 // The stretch of CTA `c`: sc->cut[0] where it begins, sc->cut[1] where it ends,
 // valid for all threads on return.  Called by the whole block.
-template <int ROWS, int KEYS, int THREADS>
+template <int KEYS, int THREADS>
 __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScratch<THREADS>* sc) {
   const int tid = threadIdx.x, lane = tid & 31;
   long long total = 0;
   for (int s0 = 0; s0 < a.b.n_seqs; s0 += THREADS) {
     long long all;
-    paged_count<ROWS, KEYS, THREADS>(a, s0, sc);
+    paged_count<KEYS, THREADS>(a, s0, sc);
     block_scan<THREADS>((long long)a.heads * sc->seq_units[tid], sc->warp_sum, &all);
     total += all;
   }
@@ -165,7 +176,7 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
   __syncthreads();
   long long before = 0;
   for (int s0 = 0; s0 < a.b.n_seqs; s0 += THREADS) {
-    if (a.b.n_seqs > THREADS) paged_count<ROWS, KEYS, THREADS>(a, s0, sc);  // else it lies there still
+    if (a.b.n_seqs > THREADS) paged_count<KEYS, THREADS>(a, s0, sc);  // else it lies there still
     const long long w = (long long)a.heads * sc->seq_units[tid];
     long long all;
     const long long at = before + block_scan<THREADS>(w, sc->warp_sum, &all);
@@ -182,13 +193,13 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
   if (tid < 64) {  // a warp for each end: the tile of its sequence
     PagedCut& k = sc->cut[tid >> 5];
     if (k.seq >= 0) {
-      const PagedSeq q = paged_seq<ROWS>(a, k.seq);
+      const PagedSeq q = paged_seq(a, k.seq);
       const long long rel = u[tid >> 5] - sc->seq_at[tid >> 5], each = sc->seq_each[tid >> 5];
       const int head = (int)(rel / each);
       const int in_head = (int)(rel - head * each);
       int begin = 0;  // units of the head before tile b0
       for (int b0 = 0; b0 < q.tiles; b0 += 32) {
-        const int n = b0 + lane < q.tiles ? paged_units<ROWS, KEYS>(a, q, b0 + lane) : 0;
+        const int n = b0 + lane < q.tiles ? paged_units<KEYS>(a, q, b0 + lane) : 0;
         int x = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -212,14 +223,13 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
 }
 
 // The tile behind (s, head, b); false at the end of the line.
-template <int ROWS>
 __device__ __forceinline__ bool paged_next(const PagedArgs& a, PagedSeq* q, int* s, int* head, int* b) {
   if (++*b < q->tiles) return true;
   *b = 0;
   if (++*head < a.heads) return true;
   *head = 0;
   while (++*s < a.b.n_seqs) {
-    *q = paged_seq<ROWS>(a, *s);
+    *q = paged_seq(a, *s);
     if (q->tiles) return true;
   }
   return false;

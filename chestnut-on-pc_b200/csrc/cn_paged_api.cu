@@ -56,13 +56,8 @@ cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tk, const CUtenso
                         cudaStream_t s) {
   static unsigned long long ready = 0;
   if (dev >= 64 || !(ready & (1ull << dev))) {
-    cudaFuncAttributes at;
-    cudaError_t e = cudaFuncGetAttributes(&at, k_paged_many<T, DIM, CODED>);
-    // the warpgroups share out 4 x 128 registers: a block that is launched with fewer would wait for ever
-    if (e == cudaSuccess && at.numRegs != 128) e = cudaErrorInvalidKernelImage;
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(k_paged_many<T, DIM, CODED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)Many<DIM>::Smem);
+    const cudaError_t e = cudaFuncSetAttribute(k_paged_many<T, DIM, CODED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)Many<DIM>::Smem);
     if (e != cudaSuccess) return e;
     if (dev < 64) ready |= 1ull << dev;
   }
@@ -114,6 +109,10 @@ int paged_check(const char* who, const cn_kv_cache* cache, const cn_kv_batch* ba
   if (q->dim != cache->dim || q->heads % cache->heads) {
     set_last_error("%s: %d query heads of %d values over %d cache heads of %d", who, q->heads, q->dim, cache->heads,
                    cache->dim);
+    return CN_ERR_ARG;
+  }
+  if (q->heads / cache->heads > 128) {
+    set_last_error("%s: %d query heads read one cache head (at most 128)", who, q->heads / cache->heads);
     return CN_ERR_ARG;
   }
   if (tokens < 0 || tokens * (q->heads / cache->heads) > (1ll << 30)) {
@@ -188,6 +187,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
   a.v_exp = cache->v_exp;
   a.heads = cache->heads;
   a.group = q->heads / cache->heads;
+  a.group_mul = a.group == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)a.group);
   a.scale = scale * 1.44269504088896340736f;
   a.causal = causal != 0;
   a.window = window;
@@ -207,6 +207,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     f.rows_min = 1;
     f.rows_max = c.do_many ? kFewRows : INT32_MAX;
     f.ctas = min(2 * sm_count(dev.device()), kFewCtas);
+    f.tile_tokens = f.half_tokens = kFewRows / a.group;
     f.min_units = f.snap = 4;
     f.cuts = reinterpret_cast<PagedCut*>(w);
     f.part_o = reinterpret_cast<float*>(w + few.o);
@@ -218,6 +219,8 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     m.rows_min = c.do_few ? kFewRows + 1 : 1;
     m.rows_max = INT32_MAX;
     m.ctas = min(sm_count(dev.device()), kManyCtas);
+    m.half_tokens = kManyRows / 2 / a.group;
+    m.tile_tokens = 2 * m.half_tokens;
     m.min_units = m.snap = 2;
     w += few.bytes;
     m.cuts = reinterpret_cast<PagedCut*>(w);

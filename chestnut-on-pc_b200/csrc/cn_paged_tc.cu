@@ -6,14 +6,17 @@
 // tensor memory (columns 0..127 and 128..255: S of the halves, P written over it
 // as 16-bit pairs; 256.. and 384..: O), so the weights never pass through shared
 // memory: P is the A operand of the second product from tensor memory.
-//   warpgroups 0, 1: softmax of a half, one thread a row, the row's 128 scores in
+// A block's S comes as two products of 64 keys.  While a half's threads are in
+// the softmax of one, the tensor core adds the other one's P V and computes its
+// next S: with one S of 128 keys a half, each block paid softmax, hand-over and
+// both products one after the other (6000 clocks a block against 3000).
+//   warpgroups 0, 1: softmax of a half, one thread a row, a row's 64 scores in
 //                    registers: no shuffles
 //   warpgroup 2:     loads.  A 16-bit cache comes by TMA, a box a page, in the
 //                    128-byte swizzle that the tensor core reads; of an 8-bit one
 //                    the threads hold the codes of the next K and V block in
 //                    registers and store them as f16 (exact) in that swizzle
-//   warp 12:         issues the products: while one half is in its softmax the
-//                    tensor core works for the other one
+//   warp 12:         issues the products
 // The running maximum is raised only when a block's exceeds it by 2^8 (the sums
 // stay exact, the weights are just up to 256): O is rescaled in tensor memory by
 // the row's own thread then, which is rare after the first blocks.
@@ -34,15 +37,6 @@ constexpr int kManyKeys = 128;
 constexpr int kManyThreads = 512;
 constexpr float kLazy = 8.f;  // the maximum may be exceeded by 2^8 before it is raised
 
-// Registers of the warpgroups; the sum is 4 x 128, what the block is launched with.
-template <bool CODED>
-struct ManyRegs {
-  static constexpr int Softmax = CODED ? 176 : 192;
-  static constexpr int Load = CODED ? 96 : 64;
-  static constexpr int Mma = 64;
-  static_assert(2 * Softmax + Load + Mma == 512, "register split");
-};
-
 template <int DIM>
 struct Many {
   static constexpr int Sub = 128 * 128;            // 128 rows x 64 values of 16 bits
@@ -53,7 +47,11 @@ struct Many {
 };
 
 struct ManyBars {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], vfix[2], sfull[2], pfull[2], ofull[2], qfull, qempty;
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], vfix[2];  // stages
+  uint64_t sfull[2][2], pfull[2][2];                           // [half][64 keys of a block]
+  uint64_t odone[2][2];                                        // its product with V is added to O
+  uint64_t asked;                                              // V of an edge block is on its way
+  uint64_t qfull, qempty;
   uint32_t tmem;
 };
 
@@ -63,34 +61,31 @@ struct ManyPart {
   int j0, j1;      // blocks of 128 keys, from lo
   int a[2], b[2];  // those that the halves take part in
   int all_lo, all_hi, hi;
-  int rows, row0;
+  int tok0, toks;  // tokens of the sequence
 };
 
 __device__ __forceinline__ ManyPart many_part(const PagedArgs& a, const PagedSeq& q, int tile, int u0, int u1) {
   ManyPart p;
-  int hi;
-  paged_range<kManyRows, kManyKeys>(a, q, tile, &p.lo, &hi);
-  p.hi = hi;
-  p.row0 = tile * kManyRows;
-  p.rows = min(q.rows - p.row0, kManyRows);
+  p.tok0 = tile * a.tile_tokens;
+  p.toks = paged_tokens(a, q, tile);
+  paged_range<kManyKeys>(a, q, p.tok0, p.toks, &p.lo, &p.hi);
   p.j0 = u0;
-  p.j1 = min(u1, max((hi - p.lo + kManyKeys - 1) / kManyKeys, u0));
+  p.j1 = min(u1, max((p.hi - p.lo + kManyKeys - 1) / kManyKeys, u0));
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     p.a[t] = p.b[t] = p.j1;
-    if (p.rows > t * 128 && p.j1 > p.j0) {
-      const int first = q.past + (p.row0 + t * 128) / a.group;
-      const int last = q.past + (min(p.row0 + t * 128 + 128, q.rows) - 1) / a.group;
-      const int thi = last < 0 ? 0 : a.causal ? min(q.len, last + 1) : q.len;
-      const int tlo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
-      if (thi > tlo) {
-        p.a[t] = max(p.j0, (tlo - p.lo) / kManyKeys);
-        p.b[t] = min(p.j1, (thi - p.lo + kManyKeys - 1) / kManyKeys);
+    const int n = min(p.toks - t * a.half_tokens, a.half_tokens);
+    if (n > 0 && p.j1 > p.j0) {
+      int lo, hi;
+      paged_range<kManyKeys>(a, q, p.tok0 + t * a.half_tokens, n, &lo, &hi);
+      if (hi > lo) {
+        p.a[t] = max(p.j0, (lo - p.lo) / kManyKeys);
+        p.b[t] = min(p.j1, (hi - p.lo + kManyKeys - 1) / kManyKeys);
         if (p.b[t] < p.a[t]) p.a[t] = p.b[t] = p.j1;
       }
     }
   }
-  const int first_pos = q.past + p.row0 / a.group, last_pos = q.past + (p.row0 + p.rows - 1) / a.group;
+  const int first_pos = q.past + p.tok0, last_pos = first_pos + p.toks - 1;
   p.all_hi = first_pos < 0 ? 0 : a.causal ? min(q.len, first_pos + 1) : q.len;
   p.all_lo = a.window > 0 ? last_pos - a.window + 1 : 0;
   return p;
@@ -102,9 +97,22 @@ __device__ __forceinline__ bool many_edge(const ManyPart& p, int j) {
   return k0 < p.all_lo || k0 + kManyKeys > p.all_hi;
 }
 
+// Bounded wait on the critical path: the limit goes by the SM's clock (%globaltimer
+// takes about as long to read as a whole block's products).
+constexpr long long kManyWaitClocks = 4000000000ll;  // ~2 s
+__device__ __forceinline__ bool many_wait1(uint64_t* bar, uint32_t parity, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > kManyWaitClocks) {
+      set_dev_error(code);
+      return false;
+    }
+  return true;
+}
 // A warp's wait: the same answer for all its lanes.
 __device__ __forceinline__ bool many_wait(uint64_t* bar, uint32_t parity, int code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+  return __all_sync(0xffffffffu, many_wait1(bar, parity, code));
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
@@ -136,14 +144,39 @@ __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
   return r;
 }
 
-// D[tmem] += A[tmem] * B[smem], 16-bit operands.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc) {
+// The products of the issuing thread.  A shared-memory descriptor's high word is
+// the same for all operands here; its low word counts 16-byte steps, so the k
+// steps are additions to it (umma_desc_sw128 anew for each costs more than the
+// product itself takes).
+constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;  // 8-row groups 1024 B apart, version 1, 128-byte swizzle
+__device__ __forceinline__ uint32_t desc_lo(const void* p, uint32_t lbo_bytes) {
+  return (smem_u32(p) >> 4) | (lbo_bytes >> 4) << 16;
+}
+// D[tmem] (+)= A[smem] * B[smem]^T, 16-bit operands.
+template <bool ADD>
+__device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.eq.u32 p, 0, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %4};\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "n"(kDescHi), "n"(ADD ? 1 : 0)
       : "memory");
+}
+// D[tmem] += A[tmem] * B[smem].
+__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "setp.eq.u32 p, 0, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "n"(kDescHi)
+      : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 
 template <typename M>
@@ -158,15 +191,12 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
   return (w & e) == e || (w & (e << 16)) == (e << 16);
 }
 
-__device__ __forceinline__ void load_group_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-
 // T: q and out (and a 16-bit cache).
 template <typename T, int DIM, bool CODED>
 __global__ void __launch_bounds__(kManyThreads, 1)
     k_paged_many(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
   using L = Many<DIM>;
   using M = std::conditional_t<CODED, __half, T>;
-  using R = ManyRegs<CODED>;
   extern __shared__ uint8_t many_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
@@ -187,12 +217,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       mbar_init(&bar.kempty[i], 1);
       mbar_init(&bar.vempty[i], 1);
       mbar_init(&bar.vfix[i], 128);
-      mbar_init(&bar.sfull[i], 1);
-      mbar_init(&bar.pfull[i], 128);
-      mbar_init(&bar.ofull[i], 1);
+      mbar_init(&bar.sfull[i][0], 1);
+      mbar_init(&bar.sfull[i][1], 1);
+      mbar_init(&bar.pfull[i][0], 128);
+      mbar_init(&bar.pfull[i][1], 128);
+      mbar_init(&bar.odone[i][0], 1);
+      mbar_init(&bar.odone[i][1], 1);
     }
     mbar_init(&bar.qfull, 128);
     mbar_init(&bar.qempty, 1);
+    mbar_init(&bar.asked, 1);
     fence_barrier_init();
     if constexpr (!CODED) {
       tma_prefetch_desc(&tm_k);
@@ -209,7 +243,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   const uint32_t tmem = bar.tmem;
   pdl_trigger();
   pdl_wait();
-  paged_find<kManyRows, kManyKeys, kManyThreads>(a, blockIdx.x, &sc);
+  paged_find<kManyKeys, kManyThreads>(a, blockIdx.x, &sc);
   if (tid == 0) a.cuts[blockIdx.x] = sc.cut[0];
   long long at = sc.cut[0].start;
   const long long end = sc.cut[1].start;
@@ -217,11 +251,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   long long first = sc.cut[0].first;
   PagedSeq q = {};
   bool more = at < end;
-  if (more) q = paged_seq<kManyRows>(a, s);
+  if (more) q = paged_seq(a, s);
   // Every role walks the same parts: advance() steps to the next one.
   int units = 0, u0 = 0, u1 = 0;
   auto part = [&]() {
-    units = paged_units<kManyRows, kManyKeys>(a, q, tile);
+    units = paged_units<kManyKeys>(a, q, tile);
     u0 = (int)(at - first);
     u1 = (int)min((long long)units, end - first);
     return many_part(a, q, tile, u0, u1);
@@ -229,22 +263,23 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   auto advance = [&]() {
     at = first + u1;
     first += units;
-    more = at < end && paged_next<kManyRows>(a, &q, &s, &head, &tile);
+    more = at < end && paged_next(a, &q, &s, &head, &tile);
   };
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::Softmax));
     const int t = warp >> 2, r = tid & 127;
+    const int my_i = div_by(r, a.group, a.group_mul), my_h = r - my_i * a.group;  // token of the half, query head
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
-    uint32_t ns = 0, no = 0, nb = 0, np = 0, fixes = 0;  // S blocks, O tiles, blocks and parts so far; fixes: phase bit of a stage
+    // so far: blocks of this half, blocks and parts of the CTA; fixes: phase bit of a stage
+    uint32_t ns = 0, nb = 0, np = 0, fixes = 0;
     bool ok = true;
     for (; more && ok; advance()) {
       const ManyPart p = part();
-      const int row = p.row0 + t * 128 + r;
-      const bool live = t * 128 + r < p.rows;
-      const int pos = live ? q.past + row / a.group : -1;
+      const int tok = t * a.half_tokens + my_i;  // of the tile
+      const bool live = my_i < a.half_tokens && tok < p.toks;
+      const int pos = live ? q.past + p.tok0 + tok : -1;
       const int see_hi = pos < 0 ? 0 : a.causal ? min(q.len, pos + 1) : q.len;
       const int see_lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
       float m = -INFINITY, l = 0.f;
@@ -258,95 +293,104 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tmem_st_wait();
       }
       float rs = 1.f;
+#pragma unroll 1
       for (int j = p.j0; j < p.j1 && ok; ++j) {
-        const uint32_t st = (nb + j - p.j0) & 1;
+        const uint32_t n = nb + j - p.j0, st = n & 1;
         const bool edge = many_edge(p, j);
         const uint32_t fix = (fixes >> st) & 1;
         if (edge) fixes ^= 1u << st;
         if (j < ja || j >= jb) continue;
-        ok = many_wait(&bar.sfull[t], ns & 1, 3);
-        if (!ok) break;
-        ++ns;
-        tc_fence_after();
-        if constexpr (CODED && std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][t * 128 + r];
-        const int k0 = p.lo + j * kManyKeys;
-        uint32_t raw[128];
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) tmem_ld32(ts + c, raw + c);
-        if (edge) {  // its V is in order, and what lies beside it
-          ok = many_wait(&bar.vfix[st], fix, 2);
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+          ok = many_wait(&bar.sfull[t][h], ns & 1, 3);
           if (!ok) break;
-        }
-        if constexpr (CODED) {
-          ok = many_wait(&bar.vfull[st], ((nb + j - p.j0) >> 1) & 1, 1);
-          if (!ok) break;
-        }
-        tmem_ld_wait();
-        float x[128];
-#pragma unroll
-        for (int c = 0; c < 128; ++c) x[c] = __uint_as_float(raw[c]);
-        if constexpr (CODED) {
-#pragma unroll
-          for (int c = 0; c < 128; c += 2) {
-            const float4 ke = *reinterpret_cast<const float4*>(kx[st][c]);
-            const float4 ve = *reinterpret_cast<const float4*>(vx[st][c]);
-            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-              x[c] *= rs;
-              x[c + 1] *= rs;
-            }
-            x[c] = fmaf(x[c], ke.x, ve.x);
-            x[c + 1] = fmaf(x[c + 1], ke.z, ve.z);
+          tc_fence_after();
+          const uint32_t th = ts + h * 64;
+          const int k0 = p.lo + j * kManyKeys + h * 64;
+          uint32_t raw[64];
+          tmem_ld32(th, raw);
+          tmem_ld32(th + 32, raw + 32);
+          if (edge && h == 0) {  // its V is in order, and what lies beside it
+            ok = many_wait(&bar.vfix[st], fix, 2);
+            if (!ok) break;
           }
-        }
-        if (edge) {
-          const int clo = see_lo - k0, chi = see_hi - k0;
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c < clo || c >= chi) x[c] = -INFINITY;
-        }
-        float mx[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx[i] = x[i];
-#pragma unroll
-        for (int c = 4; c < 128; c += 4)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], x[c + i]);
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if constexpr (!CODED) top *= a.scale;
-        const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
-        if (__any_sync(0xffffffffu, raise)) {
-          // S of this block was complete after every product before it: O stands still
-          const float c = raise ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
-          if (raise) m = top;
-          l *= c;
-          if (j > ja) {
-#pragma unroll
-            for (int d = 0; d < DIM; d += 32) {
-              uint32_t o[32];
-              tmem_ld32(to + d, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
-              tmem_st32(to + d, o);
+          if constexpr (CODED) {
+            if (h == 0) {
+              if constexpr (std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][t * 128 + r];
+              ok = many_wait(&bar.vfull[st], (n >> 1) & 1, 1);
+              if (!ok) break;
             }
           }
-        }
-        const float sub = m == -INFINITY ? 0.f : -m;
-        if (edge) {
-          // rows of V that are not finite: for the rows that see them, from the cache itself
+          tmem_ld_wait();
+          float x[64];
+#pragma unroll
+          for (int c = 0; c < 64; ++c) x[c] = __uint_as_float(raw[c]);
+          if constexpr (CODED) {
+#pragma unroll
+            for (int c = 0; c < 64; c += 2) {
+              const float4 ke = *reinterpret_cast<const float4*>(kx[st][h * 64 + c]);
+              const float4 ve = *reinterpret_cast<const float4*>(vx[st][h * 64 + c]);
+              if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+                x[c] *= rs;
+                x[c + 1] *= rs;
+              }
+              x[c] = fmaf(x[c], ke.x, ve.x);
+              x[c + 1] = fmaf(x[c + 1], ke.z, ve.z);
+            }
+          }
+          if (edge) {
+            const int clo = see_lo - k0, chi = see_hi - k0;
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (c < clo || c >= chi) x[c] = -INFINITY;
+          }
+          float mx[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = x[i];
+#pragma unroll
+          for (int c = 4; c < 64; c += 4)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], x[c + i]);
+          float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          if constexpr (!CODED) top *= a.scale;
+          const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+          const uint32_t odd = edge ? bad[st][2 * h] | bad[st][2 * h + 1] : 0u;
+          const bool begun = j > ja || h > 0;  // there are sums in O
+          const bool any = __any_sync(0xffffffffu, raise);
+          if (begun && (any || odd)) {  // O stands still once the product before this one is added
+            ok = many_wait(&bar.odone[t][h ^ 1], (ns + h + 1) & 1, 3);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          if (any) {
+            const float c = raise ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
+            if (raise) m = top;
+            l *= c;
+            if (begun) {
 #pragma unroll 1
-          for (int w = 0; w < 4; ++w) {
-            uint32_t bits = bad[st][w];
+              for (int d = 0; d < DIM; d += 32) {
+                uint32_t o[32];
+                tmem_ld32(to + d, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+                tmem_st32(to + d, o);
+              }
+            }
+          }
+          const float sub = m == -INFINITY ? 0.f : -m;
+          if (odd) {
+            // rows of V that are not finite: for the rows that see them, from the cache itself
+            tmem_st_wait();
 #pragma unroll 1
-            while (bits) {
-              const int c = w * 32 + __ffs(bits) - 1;
-              bits &= bits - 1;
-              float sx = __uint_as_float(tmem_ld1(ts + c));
+            for (int c = 0; c < 64; ++c) {
+              if (!((bad[st][2 * h + (c >> 5)] >> (c & 31)) & 1u)) continue;
+              float w = __uint_as_float(tmem_ld1(th + c));
               tmem_ld_wait();
               if constexpr (CODED)
-                sx = exp2_approx(fmaf(sx * rs, kx[st][c][0], vx[st][c][0]) + sub);
+                w = exp2_approx(fmaf(w * rs, kx[st][h * 64 + c][0], vx[st][h * 64 + c][0]) + sub);
               else
-                sx = exp2_approx(fmaf(sx, a.scale, sub));
+                w = exp2_approx(fmaf(w, a.scale, sub));
               const int key = k0 + c;
               const bool see = key >= see_lo && key < see_hi;
               const int page = page_of(a.b, s, key);
@@ -364,8 +408,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                   else
                     v = Num<T>::unpack(*reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v) + vr * DIM + d + i));
                   if (see) {
-                    o[i] = __float_as_uint(fmaf(sx, v.x, __uint_as_float(o[i])));
-                    o[i + 1] = __float_as_uint(fmaf(sx, v.y, __uint_as_float(o[i + 1])));
+                    o[i] = __float_as_uint(fmaf(w, v.x, __uint_as_float(o[i])));
+                    o[i + 1] = __float_as_uint(fmaf(w, v.y, __uint_as_float(o[i + 1])));
                   }
                 }
                 tmem_st32(to + d, o);
@@ -373,19 +417,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               tmem_st_wait();
             }
           }
-        }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 128; h += 64) {
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
           uint32_t pk[32];
 #pragma unroll
-          for (int c = h; c < h + 64; c += 4) {
+          for (int c = 0; c < 64; c += 4) {
             float e[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] = exp2_approx(CODED ? x[c + i] + sub : fmaf(x[c + i], a.scale, sub));
             if constexpr (CODED) {
-              const float4 v0 = *reinterpret_cast<const float4*>(vx[st][c]);
-              const float4 v1 = *reinterpret_cast<const float4*>(vx[st][c + 2]);
+              const float4 v0 = *reinterpret_cast<const float4*>(vx[st][h * 64 + c]);
+              const float4 v1 = *reinterpret_cast<const float4*>(vx[st][h * 64 + c + 2]);
               sum[0] = fmaf(e[0], v0.y, sum[0]);
               sum[1] = fmaf(e[1], v0.w, sum[1]);
               sum[2] = fmaf(e[2], v1.y, sum[2]);
@@ -394,15 +435,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
               for (int i = 0; i < 4; ++i) sum[i] += e[i];
             }
-            pk[(c - h) / 2] = Num<M>::pack(e[0], e[1]);
-            pk[(c - h) / 2 + 1] = Num<M>::pack(e[2], e[3]);
+            pk[c / 2] = Num<M>::pack(e[0], e[1]);
+            pk[c / 2 + 1] = Num<M>::pack(e[2], e[3]);
           }
-          tmem_st32(ts + h / 2, pk);
+          tmem_st32(th, pk);
+          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&bar.pfull[t][h]);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&bar.pfull[t]);
+        ++ns;
       }
       nb += p.j1 - p.j0;
       np += p.j1 > p.j0;
@@ -411,16 +453,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const bool complete = u0 == 0 && u1 == units;
       const long long slot = 2ll * blockIdx.x + (u0 == 0 ? 1 : 0);
       if (ja < jb) {
-        ok = many_wait(&bar.ofull[t], no & 1, 3);
-        ++no;
+        ok = many_wait(&bar.odone[t][1], (ns - 1) & 1, 3);
         if (!ok) break;
         tc_fence_after();
       }
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
-      T* out = static_cast<T*>(a.out) + (long long)(q.tok0 + row / a.group) * a.o_token +
-               (long long)(head * a.group + row % a.group) * a.o_head;
+      T* out = static_cast<T*>(a.out) + (long long)(q.tok0 + p.tok0 + tok) * a.o_token +
+               (long long)(head * a.group + my_h) * a.o_head;
       const long long pr = slot * kManyRows + t * 128 + r;
-#pragma unroll
+#pragma unroll 1
       for (int d = 0; d < DIM; d += 32) {
         uint32_t o[32];
         if (ja < jb) {
@@ -452,9 +493,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------ loads
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Load));
     const int lt = tid - 256;
-    uint32_t nb = 0, np = 0;  // blocks, parts with blocks so far
+    uint32_t nb = 0, np = 0, edges = 0;  // blocks, parts with blocks, edge blocks so far
     bool ok = true;
     const int shift = a.b.page_shift, page_rows = 1 << shift;
     const int box_rows = min(page_rows, kManyKeys);
@@ -466,7 +506,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // 16-bit cache: thread 0 asks for block j of K or V
       auto fetch = [&](int j, uint32_t n, const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty) {
         const uint32_t st = n & 1;
-        if (n >= 2 && !mbar_wait(&empty[st], ((n >> 1) & 1) ^ 1, 2)) return false;
+        if (n >= 2 && !many_wait1(&empty[st], ((n >> 1) & 1) ^ 1, 2)) return false;
         const int k0 = p.lo + j * kManyKeys;
         const int boxes = (min(kManyKeys, p.hi - k0) + box_rows - 1) / box_rows;
         uint32_t bytes = 0;
@@ -539,12 +579,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // ---- Q: 128 or 256 rows, swizzled
       if (np > 0 && ok) ok = many_wait(&bar.qempty, (np - 1) & 1, 2);
       ++np;
-      const int qrows = p.rows > 128 ? 256 : 128;
+      const int qrows = p.toks > a.half_tokens ? 256 : 128;
       constexpr int CH = DIM / 8;  // 16-byte pieces of a row
       auto q_src = [&](int i) {
-        const int row = p.row0 + min(i / CH, p.rows - 1);
-        return static_cast<const T*>(a.q) + (long long)(q.tok0 + row / a.group) * a.q_token +
-               (long long)(head * a.group + row % a.group) * a.q_head + (i % CH) * 8;
+        const int r = (i / CH) & 127, in = div_by(r, a.group, a.group_mul);
+        const int tok = min((i / CH >> 7) * a.half_tokens + in, p.toks - 1);  // rows of no token: any
+        return static_cast<const T*>(a.q) + (long long)(q.tok0 + p.tok0 + tok) * a.q_token +
+               (long long)(head * a.group + r - in * a.group) * a.q_head + (i % CH) * 8;
       };
       auto q_dst = [&](int i) {
         const int r = i / CH, ch = i % CH;
@@ -557,7 +598,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           uint4 w[4];
 #pragma unroll
           for (int x = 0; x < 4; ++x)
-            w[x] = (i0 + x * 128) / CH < p.rows ? *reinterpret_cast<const uint4*>(q_src(i0 + x * 128)) : make_uint4(0, 0, 0, 0);
+            w[x] = *reinterpret_cast<const uint4*>(q_src(i0 + x * 128));
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int i = i0 + x * 128;
@@ -583,7 +624,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
       } else {
 #pragma unroll 4
-        for (int i = lt; i < qrows * CH; i += 128) cp_async16_or_zero(smem_u32(q_dst(i)), q_src(i), i / CH < p.rows);
+        for (int i = lt; i < qrows * CH; i += 128) cp_async16(q_dst(i), q_src(i));
         cp_async_wait_all();
       }
       fence_proxy_async_smem();
@@ -626,7 +667,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           ok = __all_sync(0xffffffffu, ok);
         }
         if (edge && ok) {
+          // the other warps come here ahead of the thread that asks for the blocks: a parity says
+          // nothing about a block that is not asked for yet
+          if constexpr (!CODED) {
+            if (lt == 0) mbar_arrive(&bar.asked);
+            ok = many_wait(&bar.asked, edges & 1, 2);
+            ++edges;
+            if (!ok) break;
+          }
           ok = many_wait(&bar.vfull[st], (n >> 1) & 1, 1);
+          if (!ok) break;
           const int key = p.lo + j * kManyKeys + lt;
           uint8_t* vr = sv + st * L::Tile + lt * 128;
           bool odd = false;
@@ -660,83 +710,79 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Mma));
-    if (warp == 12 && lane == 0) {
+    if (warp == 12 && elect_one()) {
       // ------------------------------------------------------------ products
-      constexpr uint32_t id_s = many_idesc<M>(kManyKeys, false), id_o = many_idesc<M>(DIM, true);
+      constexpr uint32_t id_s = many_idesc<M>(64, false), id_o = many_idesc<M>(DIM, true);
       uint32_t nb = 0, np = 0, ns[2] = {0, 0}, fixes = 0;
       bool ok = true;
-      auto scores = [&](int t, uint32_t st) {
-        const uint32_t qa = smem_u32(sq) + t * L::Tile, ka = smem_u32(sk) + st * L::Tile;
+      const uint32_t q_lo = desc_lo(sq, 16), k_lo = desc_lo(sk, 16), v_lo = desc_lo(sv, L::Sub);
+      // S of half t and keys h * 64 .. of a block: rows h * 64 .. of the K tile
+      auto scores = [&](int t, int h, uint32_t st) {
+        const uint32_t qa = q_lo + t * (L::Tile >> 4), ka = k_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4);
+        const uint32_t d = tmem + t * 128 + h * 64;
+        tc_mma_ss<false>(d, qa, ka, id_s);
 #pragma unroll
-        for (int k = 0; k < DIM / 16; ++k) {
-          const uint32_t off = (k >> 2) * L::Sub + (k & 3) * 32;
-          tc_mma_f16(tmem + t * 128, umma_desc_sw128(qa + off, 16, 1024), umma_desc_sw128(ka + off, 16, 1024), id_s, k > 0);
+        for (int k = 1; k < DIM / 16; ++k) {
+          const uint32_t off = ((k >> 2) * L::Sub + (k & 3) * 32) >> 4;
+          tc_mma_ss<true>(d, qa + off, ka + off, id_s);
         }
-        tc_commit(&bar.sfull[t]);
+        tc_commit(&bar.sfull[t][h]);
       };
       for (; more && ok; advance()) {
         const ManyPart p = part();
         if (p.j0 >= p.j1) continue;
-        ok = mbar_wait(&bar.qfull, np & 1, 1) && mbar_wait(&bar.kfull[nb & 1], (nb >> 1) & 1, 1);
+        ok = many_wait1(&bar.qfull, np & 1, 1) && many_wait1(&bar.kfull[nb & 1], (nb >> 1) & 1, 1);
         if (!ok) break;
         ++np;
         tc_fence_after();
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (p.a[t] == p.j0 && p.a[t] < p.b[t]) scores(t, nb & 1);
+#pragma unroll 1
+        for (int x = 0; x < 4; ++x) {
+          const int ja = x & 1 ? p.a[1] : p.a[0], jb = x & 1 ? p.b[1] : p.b[0];
+          if (ja == p.j0 && ja < jb) scores(x & 1, x >> 1, nb & 1);
+        }
         tc_commit(&bar.kempty[nb & 1]);
         if (p.j1 == p.j0 + 1) tc_commit(&bar.qempty);
+#pragma unroll 1
         for (int j = p.j0; j < p.j1 && ok; ++j) {
           const uint32_t n = nb + j - p.j0, st = n & 1;
-          bool v_there = false, k_there = false;
-          auto need_v = [&]() {
-            if (v_there) return true;
-            v_there = true;
-            bool good = mbar_wait(&bar.vfull[st], (n >> 1) & 1, 1);
-            if (good && many_edge(p, j)) good = mbar_wait(&bar.vfix[st], (fixes >> st) & 1, 1);
-            return good;
-          };
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (j >= p.a[t] && j < p.b[t]) {
-              ok = ok && need_v() && mbar_wait(&bar.pfull[t], ns[t] & 1, 3);
+          ok = many_wait1(&bar.vfull[st], (n >> 1) & 1, 1);
+          if (ok && many_edge(p, j)) {
+            ok = many_wait1(&bar.vfix[st], (fixes >> st) & 1, 1);
+            fixes ^= 1u << st;
+          }
+          if (ok && j + 1 < p.j1) ok = many_wait1(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, 1);
+          if (!ok) break;
+#pragma unroll 1
+          for (int x = 0; x < 4; ++x) {
+            const int t = x & 1, h = x >> 1;
+            const int ja = t ? p.a[1] : p.a[0], jb = t ? p.b[1] : p.b[0];
+            if (j >= ja && j < jb) {
+              ok = many_wait1(&bar.pfull[t][h], (t ? ns[1] : ns[0]) & 1, 3);
               if (!ok) break;
-              ++ns[t];
               tc_fence_after();
-              const uint32_t va = smem_u32(sv) + st * L::Tile;
+              const uint32_t va = v_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4), ap = tmem + t * 128 + h * 64;
 #pragma unroll
-              for (int k = 0; k < kManyKeys / 16; ++k)
-                tc_mma_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, umma_desc_sw128(va + k * 2048, L::Sub, 1024), id_o);
-              if (j + 1 == p.b[t]) tc_commit(&bar.ofull[t]);
+              for (int k = 0; k < 4; ++k) tc_mma_ts(tmem + 256 + t * 128, ap + k * 8, va + k * (2048 >> 4), id_o);
+              tc_commit(&bar.odone[t][h]);
             }
-            if (j + 1 >= p.a[t] && j + 1 < p.b[t]) {
-              if (!k_there) {
-                k_there = true;
-                ok = ok && mbar_wait(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, 1);
-                if (!ok) break;
-                tc_fence_after();
-              }
-              scores(t, (n + 1) & 1);
-            }
+            if (j + 1 >= ja && j + 1 < jb) scores(t, h, (n + 1) & 1);
           }
           if (!ok) break;
-          if (!v_there) ok = need_v();  // a block that neither half sees: its loads end before its stage is free
+          ns[0] += j >= p.a[0] && j < p.b[0];
+          ns[1] += j >= p.a[1] && j < p.b[1];
           if (j + 1 < p.j1) {
-            if (!k_there) ok = ok && mbar_wait(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, 1);
             tc_commit(&bar.kempty[(n + 1) & 1]);
             if (j + 2 == p.j1) tc_commit(&bar.qempty);
           }
           tc_commit(&bar.vempty[st]);
-          if (many_edge(p, j)) fixes ^= 1u << st;
         }
         nb += p.j1 - p.j0;
       }
       // the last products' arrivals land before the block ends
       if (ok && np > 0) {
-        mbar_wait(&bar.kempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
-        mbar_wait(&bar.qempty, (np - 1) & 1, 3);
-        mbar_wait(&bar.vempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
+        many_wait1(&bar.kempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
+        many_wait1(&bar.qempty, (np - 1) & 1, 3);
+        many_wait1(&bar.vempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
       }
     }
     __syncwarp();

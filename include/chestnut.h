@@ -309,7 +309,7 @@ int cn_kv_read(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_head
  * Visible to the token at position p: every j < lengths[s], if `causal` j <= p
  * only, and with window > 0 (causal only) j > p - window only.  A row that sees
  * nothing is zeros, and what is not visible has no influence, whatever its value.
- * Query head h reads cache head h / (q.heads / cache.heads).  q and out alike in
+ * Query head h reads cache head h / (q.heads / cache.heads), at most 128 of them one.  q and out alike in
  * dtype (CN_F16 or CN_BF16, the cache's own unless that is CN_E4M3), heads and
  * dim; out may be q; scale positive and finite.  Statistics and sums in f32, the weights enter the product
  * with V in 16 bits.  workspace: cn_paged_attention_workspace() bytes, 256-byte
