@@ -56,8 +56,13 @@ cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tk, const CUtenso
                         cudaStream_t s) {
   static unsigned long long ready = 0;
   if (dev >= 64 || !(ready & (1ull << dev))) {
-    const cudaError_t e = cudaFuncSetAttribute(k_paged_many<T, DIM, CODED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)Many<DIM>::Smem);
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, k_paged_many<T, DIM, CODED>);
+    // the warpgroups share out 4 x 128 registers: a block launched with fewer would wait for ever
+    if (e == cudaSuccess && at.numRegs != 128) e = cudaErrorInvalidKernelImage;
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(k_paged_many<T, DIM, CODED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)Many<DIM>::Smem);
     if (e != cudaSuccess) return e;
     if (dev < 64) ready |= 1ull << dev;
   }

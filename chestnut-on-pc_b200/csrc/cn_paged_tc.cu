@@ -16,7 +16,8 @@
 //                    128-byte swizzle that the tensor core reads; of an 8-bit one
 //                    the threads hold the codes of the next K and V block in
 //                    registers and store them as f16 (exact) in that swizzle
-//   warp 12:         issues the products
+//   warps 12, 13:    issue the products of a half each, so that one half's wait
+//                    never holds up the other
 // The running maximum is raised only when a block's exceeds it by 2^8 (the sums
 // stay exact, the weights are just up to 256): O is rescaled in tensor memory by
 // the row's own thread then, which is rare after the first blocks.
@@ -36,6 +37,15 @@ constexpr int kManyRows = 256;
 constexpr int kManyKeys = 128;
 constexpr int kManyThreads = 512;
 constexpr float kLazy = 8.f;  // the maximum may be exceeded by 2^8 before it is raised
+
+// Registers of the warpgroups (softmax, loads, products): their sum is 4 x 128, what the block is launched with.
+template <bool CODED>
+struct ManyRegs {
+  static constexpr int Softmax = CODED ? 176 : 192;
+  static constexpr int Load = CODED ? 96 : 64;
+  static constexpr int Mma = 64;
+  static_assert(2 * Softmax + Load + Mma == 512, "register split");
+};
 
 template <int DIM>
 struct Many {
@@ -137,10 +147,52 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+// Waits for this warp's tensor-memory loads.  r passes through it, so that nothing of r is read before.
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                 "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+// Pairs of f32: one instruction for two values.
+__device__ __forceinline__ uint64_t pair2(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) { return pair2(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float2 unpair2(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {  // waits too
   uint32_t r;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\ttcgen05.wait::ld.sync.aligned;" : "=r"(r) : "r"(taddr) : "memory");
   return r;
 }
 
@@ -197,6 +249,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     k_paged_many(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
   using L = Many<DIM>;
   using M = std::conditional_t<CODED, __half, T>;
+  using R = ManyRegs<CODED>;
   extern __shared__ uint8_t many_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(many_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = smem;
@@ -205,8 +258,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __shared__ PagedScratch<kManyThreads> sc;
   __shared__ ManyBars bar;
   __shared__ uint32_t bad[2][4];                        // V rows of an edge block that are not finite
-  __shared__ __align__(16) float kx[CODED ? 2 : 1][CODED ? 128 : 1][2];  // (scale 2^ek, -) of a K block
-  __shared__ __align__(16) float vx[CODED ? 2 : 1][CODED ? 128 : 1][2];  // (ev, 2^-ev) of a V block
+  // 8-bit cache, of each pair of keys: {scale 2^ek, scale 2^ek'}, {ev, ev'}; and {2^-ev, 2^-ev'}
+  __shared__ __align__(16) float kvx[CODED ? 2 : 1][CODED ? 64 : 1][2][2];
+  __shared__ __align__(16) float vback[CODED ? 2 : 1][CODED ? 64 : 1][2];
   __shared__ float qpow[2][CODED ? kManyRows : 1];      // power of two that a row of Q was divided by (parts in turn)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -214,8 +268,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.kfull[i], CODED ? 128 : 1);
       mbar_init(&bar.vfull[i], CODED ? 128 : 1);
-      mbar_init(&bar.kempty[i], 1);
-      mbar_init(&bar.vempty[i], 1);
+      mbar_init(&bar.kempty[i], 2);
+      mbar_init(&bar.vempty[i], 2);
       mbar_init(&bar.vfix[i], 128);
       mbar_init(&bar.sfull[i][0], 1);
       mbar_init(&bar.sfull[i][1], 1);
@@ -225,7 +279,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       mbar_init(&bar.odone[i][1], 1);
     }
     mbar_init(&bar.qfull, 128);
-    mbar_init(&bar.qempty, 1);
+    mbar_init(&bar.qempty, 2);
     mbar_init(&bar.asked, 1);
     fence_barrier_init();
     if constexpr (!CODED) {
@@ -233,7 +287,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       tma_prefetch_desc(&tm_v);
     }
   }
-  if (warp == 13) {
+  if (warp == 14) {
     tmem_alloc(&bar.tmem, 512);
     tmem_relinquish();
   }
@@ -268,6 +322,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R::Softmax));
     const int t = warp >> 2, r = tid & 127;
     const int my_i = div_by(r, a.group, a.group_mul), my_h = r - my_i * a.group;  // token of the half, query head
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -307,12 +362,24 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           tc_fence_after();
           const uint32_t th = ts + h * 64;
           const int k0 = p.lo + j * kManyKeys + h * 64;
-          uint32_t raw[64];
-          tmem_ld32(th, raw);
-          tmem_ld32(th + 32, raw + 32);
-          if (edge && h == 0) {  // its V is in order, and what lies beside it
-            ok = many_wait(&bar.vfix[st], fix, 2);
-            if (!ok) break;
+          if (edge) {
+            if (h == 0) {  // its V is in order, and what lies beside it
+              ok = many_wait(&bar.vfix[st], fix, 2);
+              if (!ok) break;
+            }
+            // what a row does not see becomes -inf in tensor memory; all else goes on as everywhere
+            const int clo = see_lo - k0, chi = see_hi - k0;
+#pragma unroll 1
+            for (int c0 = 0; c0 < 64; c0 += 32) {
+              uint32_t y[32];
+              tmem_ld32(th + c0, y);
+              tmem_ld_wait32(y);
+#pragma unroll
+              for (int c = 0; c < 32; ++c)
+                if (c0 + c < clo || c0 + c >= chi) y[c] = 0xff800000u;
+              tmem_st32(th + c0, y);
+            }
+            tmem_st_wait();
           }
           if constexpr (CODED) {
             if (h == 0) {
@@ -321,36 +388,42 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               if (!ok) break;
             }
           }
-          tmem_ld_wait();
-          float x[64];
-#pragma unroll
-          for (int c = 0; c < 64; ++c) x[c] = __uint_as_float(raw[c]);
+          uint32_t s0[32], s1[32];
+          tmem_ld32(th, s0);
+          tmem_ld32(th + 32, s1);
+          tmem_ld_wait32(s0);
+          tmem_ld_wait32(s1);
           if constexpr (CODED) {
+            const uint64_t rs2 = pair2(rs, rs);
+            auto to_powers = [&](uint32_t* y, int c0) {
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-              const float4 ke = *reinterpret_cast<const float4*>(kx[st][h * 64 + c]);
-              const float4 ve = *reinterpret_cast<const float4*>(vx[st][h * 64 + c]);
-              if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-                x[c] *= rs;
-                x[c + 1] *= rs;
+              for (int c = 0; c < 32; c += 2) {
+                const ulonglong2 kv = *reinterpret_cast<const ulonglong2*>(kvx[st][(h * 64 + c0 + c) / 2][0]);
+                uint64_t v = pair2(y[c], y[c + 1]);
+                if constexpr (std::is_same_v<T, __nv_bfloat16>) v = mul2(v, rs2);
+                const float2 f = unpair2(fma2(v, kv.x, kv.y));
+                y[c] = __float_as_uint(f.x);
+                y[c + 1] = __float_as_uint(f.y);
               }
-              x[c] = fmaf(x[c], ke.x, ve.x);
-              x[c + 1] = fmaf(x[c + 1], ke.z, ve.z);
-            }
-          }
-          if (edge) {
-            const int clo = see_lo - k0, chi = see_hi - k0;
-#pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (c < clo || c >= chi) x[c] = -INFINITY;
+            };
+            to_powers(s0, 0);
+            to_powers(s1, 32);
           }
           float mx[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = x[i];
+          for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s0[i]);
 #pragma unroll
-          for (int c = 4; c < 64; c += 4)
+          for (int c = 4; c < 28; c += 8)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], x[c + i]);
+            for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s0[c + i]), __uint_as_float(s0[c + 4 + i]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s0[28 + i]), __uint_as_float(s1[i]));
+#pragma unroll
+          for (int c = 4; c < 28; c += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s1[c + i]), __uint_as_float(s1[c + 4 + i]));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], __uint_as_float(s1[28 + i]));
           float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if constexpr (!CODED) top *= a.scale;
           const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
@@ -371,7 +444,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               for (int d = 0; d < DIM; d += 32) {
                 uint32_t o[32];
                 tmem_ld32(to + d, o);
-                tmem_ld_wait();
+                tmem_ld_wait32(o);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
                 tmem_st32(to + d, o);
@@ -386,9 +459,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             for (int c = 0; c < 64; ++c) {
               if (!((bad[st][2 * h + (c >> 5)] >> (c & 31)) & 1u)) continue;
               float w = __uint_as_float(tmem_ld1(th + c));
-              tmem_ld_wait();
               if constexpr (CODED)
-                w = exp2_approx(fmaf(w * rs, kx[st][h * 64 + c][0], vx[st][h * 64 + c][0]) + sub);
+                w = exp2_approx(fmaf(w * rs, kvx[st][(h * 64 + c) >> 1][0][c & 1], kvx[st][(h * 64 + c) >> 1][1][c & 1]) + sub);
               else
                 w = exp2_approx(fmaf(w, a.scale, sub));
               const int key = k0 + c;
@@ -399,7 +471,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               for (int d = 0; d < DIM; d += 32) {
                 uint32_t o[32];
                 tmem_ld32(to + d, o);
-                tmem_ld_wait();
+                tmem_ld_wait32(o);
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
                   float2 v;
@@ -417,29 +489,40 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               tmem_st_wait();
             }
           }
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint64_t sum[2] = {0ull, 0ull};
+          const uint64_t scale2 = pair2(CODED ? 1.f : a.scale, CODED ? 1.f : a.scale), sub2 = pair2(sub, sub);
           uint32_t pk[32];
+          // 16 values at a time: independent of one another, so that the exponentials follow each other closely
+          auto weigh = [&](const uint32_t* y, uint32_t* w, int c0) {
 #pragma unroll
-          for (int c = 0; c < 64; c += 4) {
-            float e[4];
+            for (int c = 0; c < 32; c += 16) {
+              float2 e[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = exp2_approx(CODED ? x[c + i] + sub : fmaf(x[c + i], a.scale, sub));
-            if constexpr (CODED) {
-              const float4 v0 = *reinterpret_cast<const float4*>(vx[st][h * 64 + c]);
-              const float4 v1 = *reinterpret_cast<const float4*>(vx[st][h * 64 + c + 2]);
-              sum[0] = fmaf(e[0], v0.y, sum[0]);
-              sum[1] = fmaf(e[1], v0.w, sum[1]);
-              sum[2] = fmaf(e[2], v1.y, sum[2]);
-              sum[3] = fmaf(e[3], v1.w, sum[3]);
-            } else {
+              for (int i = 0; i < 8; ++i) {
+                const uint64_t v = pair2(y[c + 2 * i], y[c + 2 * i + 1]);
+                e[i] = unpair2(CODED ? add2(v, sub2) : fma2(v, scale2, sub2));
+              }
 #pragma unroll
-              for (int i = 0; i < 4; ++i) sum[i] += e[i];
+              for (int i = 0; i < 8; ++i) {
+                e[i].x = exp2_approx(e[i].x);
+                e[i].y = exp2_approx(e[i].y);
+              }
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint64_t v = pair2(e[i].x, e[i].y);
+                if constexpr (CODED)
+                  sum[i & 1] = fma2(v, *reinterpret_cast<const uint64_t*>(vback[st][(h * 64 + c0 + c) / 2 + i]), sum[i & 1]);
+                else
+                  sum[i & 1] = add2(v, sum[i & 1]);
+                w[c / 2 + i] = Num<M>::pack(e[i].x, e[i].y);
+              }
             }
-            pk[c / 2] = Num<M>::pack(e[0], e[1]);
-            pk[c / 2 + 1] = Num<M>::pack(e[2], e[3]);
-          }
+          };
+          weigh(s0, pk, 0);
+          weigh(s1, pk + 16, 32);
           tmem_st32(th, pk);
-          l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+          const float2 sums = unpair2(add2(sum[0], sum[1]));
+          l += sums.x + sums.y;
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(&bar.pfull[t][h]);
@@ -466,7 +549,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         uint32_t o[32];
         if (ja < jb) {
           tmem_ld32(to + d, o);
-          tmem_ld_wait();
+          tmem_ld_wait32(o);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
@@ -493,6 +576,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------ loads
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Load));
     const int lt = tid - 256;
     uint32_t nb = 0, np = 0, edges = 0;  // blocks, parts with blocks, edge blocks so far
     bool ok = true;
@@ -638,12 +722,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if constexpr (CODED) {
           if (n >= 2) ok = many_wait(&bar.kempty[st], ((n >> 1) & 1) ^ 1, 2);
           if (!ok) break;
-          // kx and vx of a stage are read by the softmax of its block, which is over when its
+          // kvx and vback of a stage are read by the softmax of its block, which is over when its
           // products with V are: kempty alone would not say so
           if (n >= 2) ok = many_wait(&bar.vempty[st], ((n >> 1) & 1) ^ 1, 2);
           if (!ok) break;
           put(ck, sk + st * L::Tile);
-          kx[st][lt][0] = exp_byte(ek) * a.scale;
+          kvx[st][lt >> 1][0][lt & 1] = exp_byte(ek) * a.scale;
           fence_proxy_async_smem();
           mbar_arrive(&bar.kfull[st]);
           if (i + 1 < blocks) {
@@ -651,8 +735,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             ek = hold_exp(j + 1, a.k_exp);
           }
           put(cv, sv + st * L::Tile);
-          vx[st][lt][0] = (float)((int)ev - 127);
-          vx[st][lt][1] = exp_byte(254u - ev);
+          kvx[st][lt >> 1][1][lt & 1] = (float)((int)ev - 127);
+          vback[st][lt >> 1][lt & 1] = exp_byte(254u - ev);
           fence_proxy_async_smem();
           mbar_arrive(&bar.vfull[st]);
           if (i + 1 < blocks) {
@@ -710,40 +794,42 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
     }
   } else {
-    if (warp == 12 && elect_one()) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Mma));
+    if (warp < 14 && elect_one()) {
       // ------------------------------------------------------------ products
       constexpr uint32_t id_s = many_idesc<M>(64, false), id_o = many_idesc<M>(DIM, true);
-      uint32_t nb = 0, np = 0, ns[2] = {0, 0}, fixes = 0;
+      const int t = warp - 12;
+      uint32_t nb = 0, np = 0, ns = 0, fixes = 0;
       bool ok = true;
-      const uint32_t q_lo = desc_lo(sq, 16), k_lo = desc_lo(sk, 16), v_lo = desc_lo(sv, L::Sub);
-      // S of half t and keys h * 64 .. of a block: rows h * 64 .. of the K tile
-      auto scores = [&](int t, int h, uint32_t st) {
-        const uint32_t qa = q_lo + t * (L::Tile >> 4), ka = k_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4);
-        const uint32_t d = tmem + t * 128 + h * 64;
-        tc_mma_ss<false>(d, qa, ka, id_s);
+      const uint32_t q_lo = desc_lo(sq + t * L::Tile, 16), k_lo = desc_lo(sk, 16), v_lo = desc_lo(sv, L::Sub);
+      const uint32_t d_s = tmem + t * 128, d_o = tmem + 256 + t * 128;
+      // S of keys h * 64 .. of a block: rows h * 64 .. of the K tile
+      auto scores = [&](int h, uint32_t st) {
+        const uint32_t ka = k_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4);
+        tc_mma_ss<false>(d_s + h * 64, q_lo, ka, id_s);
 #pragma unroll
         for (int k = 1; k < DIM / 16; ++k) {
           const uint32_t off = ((k >> 2) * L::Sub + (k & 3) * 32) >> 4;
-          tc_mma_ss<true>(d, qa + off, ka + off, id_s);
+          tc_mma_ss<true>(d_s + h * 64, q_lo + off, ka + off, id_s);
         }
         tc_commit(&bar.sfull[t][h]);
       };
       for (; more && ok; advance()) {
         const ManyPart p = part();
         if (p.j0 >= p.j1) continue;
+        const int ja = t ? p.a[1] : p.a[0], jb = t ? p.b[1] : p.b[0];
         ok = many_wait1(&bar.qfull, np & 1, 1) && many_wait1(&bar.kfull[nb & 1], (nb >> 1) & 1, 1);
         if (!ok) break;
         ++np;
         tc_fence_after();
-#pragma unroll 1
-        for (int x = 0; x < 4; ++x) {
-          const int ja = x & 1 ? p.a[1] : p.a[0], jb = x & 1 ? p.b[1] : p.b[0];
-          if (ja == p.j0 && ja < jb) scores(x & 1, x >> 1, nb & 1);
+        if (ja == p.j0 && ja < jb) {
+          scores(0, nb & 1);
+          scores(1, nb & 1);
         }
         tc_commit(&bar.kempty[nb & 1]);
         if (p.j1 == p.j0 + 1) tc_commit(&bar.qempty);
 #pragma unroll 1
-        for (int j = p.j0; j < p.j1 && ok; ++j) {
+        for (int j = p.j0; j < p.j1; ++j) {
           const uint32_t n = nb + j - p.j0, st = n & 1;
           ok = many_wait1(&bar.vfull[st], (n >> 1) & 1, 1);
           if (ok && many_edge(p, j)) {
@@ -753,23 +839,20 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           if (ok && j + 1 < p.j1) ok = many_wait1(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, 1);
           if (!ok) break;
 #pragma unroll 1
-          for (int x = 0; x < 4; ++x) {
-            const int t = x & 1, h = x >> 1;
-            const int ja = t ? p.a[1] : p.a[0], jb = t ? p.b[1] : p.b[0];
+          for (int h = 0; h < 2; ++h) {
             if (j >= ja && j < jb) {
-              ok = many_wait1(&bar.pfull[t][h], (t ? ns[1] : ns[0]) & 1, 3);
+              ok = many_wait1(&bar.pfull[t][h], ns & 1, 3);
               if (!ok) break;
               tc_fence_after();
-              const uint32_t va = v_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4), ap = tmem + t * 128 + h * 64;
+              const uint32_t va = v_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) tc_mma_ts(tmem + 256 + t * 128, ap + k * 8, va + k * (2048 >> 4), id_o);
+              for (int k = 0; k < 4; ++k) tc_mma_ts(d_o, d_s + h * 64 + k * 8, va + k * (2048 >> 4), id_o);
               tc_commit(&bar.odone[t][h]);
             }
-            if (j + 1 >= ja && j + 1 < jb) scores(t, h, (n + 1) & 1);
+            if (j + 1 >= ja && j + 1 < jb) scores(h, (n + 1) & 1);
           }
           if (!ok) break;
-          ns[0] += j >= p.a[0] && j < p.b[0];
-          ns[1] += j >= p.a[1] && j < p.b[1];
+          ns += j >= ja && j < jb;
           if (j + 1 < p.j1) {
             tc_commit(&bar.kempty[(n + 1) & 1]);
             if (j + 2 == p.j1) tc_commit(&bar.qempty);
@@ -790,7 +873,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   // Every product's result was waited for by the softmax that used it; the others (a give-up) end here.
   tc_fence_before();
   __syncthreads();
-  if (warp == 13) {
+  if (warp == 14) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
