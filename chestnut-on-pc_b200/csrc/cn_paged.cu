@@ -113,11 +113,11 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
   const int page_rows = 1 << a.b.page_shift;
 
   while (true) {
-    const int units = paged_units<kFewKeys>(a, sq, b);
+    const int units = paged_blocks<kFewKeys>(a, sq, b);
     int lo, hi;
     const int tok0 = b * a.tile_tokens, toks = paged_tokens(a, sq, b);
     paged_range<kFewKeys>(a, sq, tok0, toks, &lo, &hi);
-    const int u0 = (int)(at - first), u1 = (int)min((long long)units, end - first);
+    const int u0 = paged_block_at(a, at, first, units), u1 = paged_block_at(a, end, first, units);
     const int rows = toks * a.group;
     auto token_of = [&](int r) { return div_by(r, a.group, a.group_mul); };
     // positions of this thread's rows g and g + 8; none: -1 sees nothing
@@ -469,9 +469,9 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kFewRows + r) * 2) = make_float2(m, l);
       }
     }
-    at = first + u1;
+    first += units + a.extra;
+    at = first;
     if (at >= end) break;
-    first += units;
     if (!paged_next(a, &sq, &s, &head, &b)) break;
     __syncthreads();  // the join's memory becomes rings again
   }

@@ -10,8 +10,10 @@
 // them.  A stretch that covers a whole tile writes its rows out; a cut tile
 // leaves (unnormalised sums, maximum, sum of weights) of each part in the
 // workspace, and k_paged_merge adds the parts up in their order, so results do
-// not depend on timing.  Tiles of at most `snap` units are never cut: a cut
-// inside one moves to its start.
+// not depend on timing.  A tile counts `extra` units more than it has, for what
+// it costs to begin and end (a CTA of the first, short tiles of a causal prompt
+// would else be the last to finish, by a third).  Tiles of at most `snap` units
+// are never cut, nor is one within its first `extra`: the cut moves to its start.
 // Everything is derived on the device from the batch's arrays (each CTA finds
 // its stretch with one scan), so a captured graph replays with new lengths.
 #pragma once
@@ -32,14 +34,14 @@ struct PagedArgs {
   float scale;          // the caller's scale * log2(e)
   int causal, window;
   int rows_min, rows_max;  // this launch takes the sequences with rows in [rows_min, rows_max]
-  int ctas, min_units, snap;
+  int ctas, min_units, snap, extra;
   struct PagedCut* cuts;   // [ctas + 1]
   float* part_o;           // [2 * ctas][ROWS][DIM]
   float* part_ml;          // [2 * ctas][ROWS][2]
 };
 
 // Where CTA c's stretch begins: unit `start` of the line, inside tile (seq,
-// head, tile), which covers [first, first + units).
+// head, tile), which covers [first, first + units), its `extra` ahead of the others.
 struct PagedCut {
   long long start, first, total;
   int seq, head, tile, units;
@@ -83,12 +85,21 @@ __device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedSeq& 
   *lo = a.window > 0 ? max(first - a.window + 1, 0) / KEYS * KEYS : 0;
 }
 
-// Units of tile b: at least one, so that rows without keys are written too.
+// Blocks of keys of tile b: at least one, so that rows without keys are written too.
 template <int KEYS>
-__device__ __forceinline__ int paged_units(const PagedArgs& a, const PagedSeq& q, int b) {
+__device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& q, int b) {
   int lo, hi;
   paged_range<KEYS>(a, q, b * a.tile_tokens, paged_tokens(a, q, b), &lo, &hi);
   return max((hi - lo + KEYS - 1) / KEYS, 1);
+}
+// Units that it counts.
+template <int KEYS>
+__device__ __forceinline__ int paged_units(const PagedArgs& a, const PagedSeq& q, int b) {
+  return paged_blocks<KEYS>(a, q, b) + a.extra;
+}
+// Block at which unit `at` of the line begins, in a tile from `first` on with n blocks.
+__device__ __forceinline__ int paged_block_at(const PagedArgs& a, long long at, long long first, int n) {
+  return (int)min(max(at - first - a.extra, 0ll), (long long)n);
 }
 
 // Sum over the block; `scratch` has a long long for each warp.
@@ -212,7 +223,7 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
           k.tile = b0 + lane;
           k.first = sc->seq_at[tid >> 5] + head * each + begin + x - n;
           k.units = n;
-          k.start = n <= a.snap ? k.first : u[tid >> 5];
+          k.start = n - a.extra <= a.snap || u[tid >> 5] - k.first <= a.extra ? k.first : u[tid >> 5];
         }
         if (__any_sync(0xffffffffu, here)) break;
         begin += __shfl_sync(0xffffffffu, x, 31);

@@ -214,6 +214,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     f.ctas = min(2 * sm_count(dev.device()), kFewCtas);
     f.tile_tokens = f.half_tokens = kFewRows / a.group;
     f.min_units = f.snap = 4;
+    f.extra = 1;
     f.cuts = reinterpret_cast<PagedCut*>(w);
     f.part_o = reinterpret_cast<float*>(w + few.o);
     f.part_ml = reinterpret_cast<float*>(w + few.ml);
@@ -227,6 +228,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     m.half_tokens = kManyRows / 2 / a.group;
     m.tile_tokens = 2 * m.half_tokens;
     m.min_units = m.snap = 2;
+    m.extra = 2;
     w += few.bytes;
     m.cuts = reinterpret_cast<PagedCut*>(w);
     m.part_o = reinterpret_cast<float*>(w + many.o);

@@ -16,6 +16,7 @@
 //                    128-byte swizzle that the tensor core reads; of an 8-bit one
 //                    the threads hold the codes of the next K and V block in
 //                    registers and store them as f16 (exact) in that swizzle
+//   warp 15:         works out the parts ahead of the others (ring of two)
 //   warps 12, 13:    issue the products of a half each, so that one half's wait
 //                    never holds up the other
 // The running maximum is raised only when a block's exceeds it by 2^8 (the sums
@@ -62,6 +63,7 @@ struct ManyBars {
   uint64_t odone[2][2];                                        // its product with V is added to O
   uint64_t asked;                                              // V of an edge block is on its way
   uint64_t qfull, qempty;
+  uint64_t told[2], heard[2];                                  // parts: worked out, read by all
   uint32_t tmem;
 };
 
@@ -72,10 +74,22 @@ struct ManyPart {
   int a[2], b[2];  // those that the halves take part in
   int all_lo, all_hi, hi;
   int tok0, toks;  // tokens of the sequence
+  int seq, head, seq_tok0, past, len;
+  int whole, first_part;  // the whole tile; its beginning
+  int live;               // 0: no further part
 };
 
-__device__ __forceinline__ ManyPart many_part(const PagedArgs& a, const PagedSeq& q, int tile, int u0, int u1) {
+__device__ __forceinline__ ManyPart many_part(const PagedArgs& a, const PagedSeq& q, int s, int head, int tile, int u0,
+                                              int u1, int units) {
   ManyPart p;
+  p.seq = s;
+  p.head = head;
+  p.seq_tok0 = q.tok0;
+  p.past = q.past;
+  p.len = q.len;
+  p.whole = u0 == 0 && u1 == units;
+  p.first_part = u0 == 0;
+  p.live = 1;
   p.tok0 = tile * a.tile_tokens;
   p.toks = paged_tokens(a, q, tile);
   paged_range<kManyKeys>(a, q, p.tok0, p.toks, &p.lo, &p.hi);
@@ -204,6 +218,22 @@ constexpr uint32_t kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;  // 8-row group
 __device__ __forceinline__ uint32_t desc_lo(const void* p, uint32_t lbo_bytes) {
   return (smem_u32(p) >> 4) | (lbo_bytes >> 4) << 16;
 }
+// 64 bytes of a thread's own row; in whole 32-byte sectors where the row allows.
+__device__ __forceinline__ void st_row64(void* p, const uint32_t* w, bool wide) {
+  if (wide) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(static_cast<uint8_t*>(p) + i * 4),
+                   "r"(w[i]), "r"(w[i + 1]), "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]),
+                   "r"(w[i + 7])
+                   : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p) + i * 4) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  }
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T, 16-bit operands.
 template <bool ADD>
 __device__ __forceinline__ void tc_mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
@@ -257,6 +287,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   uint8_t* sv = sk + L::Stages * L::Tile;
   __shared__ PagedScratch<kManyThreads> sc;
   __shared__ ManyBars bar;
+  __shared__ ManyPart parts[2];
   __shared__ uint32_t bad[2][4];                        // V rows of an edge block that are not finite
   // 8-bit cache, of each pair of keys: {scale 2^ek, scale 2^ek'}, {ev, ev'}; and {2^-ev, 2^-ev'}
   __shared__ __align__(16) float kvx[CODED ? 2 : 1][CODED ? 64 : 1][2][2];
@@ -275,6 +306,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       mbar_init(&bar.sfull[i][1], 1);
       mbar_init(&bar.pfull[i][0], 128);
       mbar_init(&bar.pfull[i][1], 128);
+      mbar_init(&bar.told[i], 1);
+      mbar_init(&bar.heard[i], 14);  // 8 softmax warps, 4 of the loads, 2 of the products
       mbar_init(&bar.odone[i][0], 1);
       mbar_init(&bar.odone[i][1], 1);
     }
@@ -299,26 +332,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   pdl_wait();
   paged_find<kManyKeys, kManyThreads>(a, blockIdx.x, &sc);
   if (tid == 0) a.cuts[blockIdx.x] = sc.cut[0];
-  long long at = sc.cut[0].start;
-  const long long end = sc.cut[1].start;
-  int s = sc.cut[0].seq, head = sc.cut[0].head, tile = sc.cut[0].tile;
-  long long first = sc.cut[0].first;
-  PagedSeq q = {};
-  bool more = at < end;
-  if (more) q = paged_seq(a, s);
-  // Every role walks the same parts: advance() steps to the next one.
-  int units = 0, u0 = 0, u1 = 0;
-  auto part = [&]() {
-    units = paged_units<kManyKeys>(a, q, tile);
-    u0 = (int)(at - first);
-    u1 = (int)min((long long)units, end - first);
-    return many_part(a, q, tile, u0, u1);
+  // Every role walks the same parts: the next one, false at the end (or where the wait was given up).
+  uint32_t np_read = 0;
+  ManyPart p;
+  auto next_part = [&]() {
+    const uint32_t i = np_read & 1;
+    if (!many_wait1(&bar.told[i], (np_read >> 1) & 1, 1)) return false;
+    p = parts[i];
+    ++np_read;
+    return p.live != 0;
   };
-  auto advance = [&]() {
-    at = first + u1;
-    first += units;
-    more = at < end && paged_next(a, &q, &s, &head, &tile);
-  };
+  // its copy in shared memory may be written anew (a warp's lane, or its only thread)
+  auto part_read = [&]() { mbar_arrive(&bar.heard[(np_read - 1) & 1]); };
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
@@ -330,15 +355,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     // so far: blocks of this half, blocks and parts of the CTA; fixes: phase bit of a stage
     uint32_t ns = 0, nb = 0, np = 0, fixes = 0;
     bool ok = true;
-    for (; more && ok; advance()) {
-      const ManyPart p = part();
+    while (ok) {
+      if (!__all_sync(0xffffffffu, next_part())) break;
+      __syncwarp();
+      if (lane == 0) part_read();
       const int tok = t * a.half_tokens + my_i;  // of the tile
       const bool live = my_i < a.half_tokens && tok < p.toks;
-      const int pos = live ? q.past + p.tok0 + tok : -1;
-      const int see_hi = pos < 0 ? 0 : a.causal ? min(q.len, pos + 1) : q.len;
+      const int pos = live ? p.past + p.tok0 + tok : -1;
+      const int see_hi = pos < 0 ? 0 : a.causal ? min(p.len, pos + 1) : p.len;
       const int see_lo = a.window > 0 ? max(pos - a.window + 1, 0) : 0;
       float m = -INFINITY, l = 0.f;
-      const int ja = p.a[t], jb = p.b[t];
+      const int ja = t ? p.a[1] : p.a[0], jb = t ? p.b[1] : p.b[0];
       if (ja < jb) {
         uint32_t z[32];
 #pragma unroll
@@ -465,8 +492,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 w = exp2_approx(fmaf(w, a.scale, sub));
               const int key = k0 + c;
               const bool see = key >= see_lo && key < see_hi;
-              const int page = page_of(a.b, s, key);
-              const long long vr = (((long long)max(page, 0) * a.heads + head) << a.b.page_shift) + (key & ((1 << a.b.page_shift) - 1));
+              const int page = page_of(a.b, p.seq, key);
+              const long long vr = (((long long)max(page, 0) * a.heads + p.head) << a.b.page_shift) + (key & ((1 << a.b.page_shift) - 1));
 #pragma unroll 1
               for (int d = 0; d < DIM; d += 32) {
                 uint32_t o[32];
@@ -533,17 +560,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       np += p.j1 > p.j0;
       if (!ok) break;
       // ---- out, or this part's sums
-      const bool complete = u0 == 0 && u1 == units;
-      const long long slot = 2ll * blockIdx.x + (u0 == 0 ? 1 : 0);
+      const long long slot = 2ll * blockIdx.x + p.first_part;
       if (ja < jb) {
         ok = many_wait(&bar.odone[t][1], (ns - 1) & 1, 3);
         if (!ok) break;
         tc_fence_after();
       }
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
-      T* out = static_cast<T*>(a.out) + (long long)(q.tok0 + p.tok0 + tok) * a.o_token +
-               (long long)(head * a.group + my_h) * a.o_head;
+      T* out = static_cast<T*>(a.out) + (long long)(p.seq_tok0 + p.tok0 + tok) * a.o_token +
+               (long long)(p.head * a.group + my_h) * a.o_head;
       const long long pr = slot * kManyRows + t * 128 + r;
+      const bool wide = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
 #pragma unroll 1
       for (int d = 0; d < DIM; d += 32) {
         uint32_t o[32];
@@ -555,23 +582,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
         if (live) {
-          if (complete) {
+          if (p.whole) {
+            uint32_t w[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = Num<T>::pack(__uint_as_float(o[i + 2 * e]) * inv, __uint_as_float(o[i + 2 * e + 1]) * inv);
-              *reinterpret_cast<uint4*>(out + d + i) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int i = 0; i < 16; ++i)
+              w[i] = Num<T>::pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            st_row64(out + d, w, wide);
           } else {
-#pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4*>(a.part_o + pr * DIM + d + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            st_row64(a.part_o + pr * DIM + d, o, true);
+            st_row64(a.part_o + pr * DIM + d + 16, o + 16, true);
           }
         }
       }
-      if (live && !complete) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(m, l);
+      if (live && !p.whole) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(m, l);
       tc_fence_before();  // the next part's zeros and products come after these loads
     }
   } else if (warp < 12) {
@@ -582,8 +605,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     bool ok = true;
     const int shift = a.b.page_shift, page_rows = 1 << shift;
     const int box_rows = min(page_rows, kManyKeys);
-    for (; more && ok; advance()) {
-      const ManyPart p = part();
+    while (ok) {
+      if (!__all_sync(0xffffffffu, next_part())) break;
+      __syncwarp();
+      if (lane == 0) part_read();
       if (p.j0 >= p.j1) continue;
       const int blocks = p.j1 - p.j0;
 
@@ -594,12 +619,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const int k0 = p.lo + j * kManyKeys;
         const int boxes = (min(kManyKeys, p.hi - k0) + box_rows - 1) / box_rows;
         uint32_t bytes = 0;
-        for (int i = 0; i < boxes; ++i) bytes += page_of(a.b, s, k0 + i * box_rows) >= 0 ? box_rows * DIM * 2 : 0;
+        for (int i = 0; i < boxes; ++i) bytes += page_of(a.b, p.seq, k0 + i * box_rows) >= 0 ? box_rows * DIM * 2 : 0;
         mbar_arrive_expect_tx(&full[st], bytes);
         for (int i = 0; i < boxes; ++i) {
-          const int page = page_of(a.b, s, k0 + i * box_rows);
+          const int page = page_of(a.b, p.seq, k0 + i * box_rows);
           if (page < 0) continue;
-          const int y = head * page_rows + ((k0 + i * box_rows) & (page_rows - 1));
+          const int y = p.head * page_rows + ((k0 + i * box_rows) & (page_rows - 1));
 #pragma unroll
           for (int d = 0; d < DIM / 64; ++d)
             tma_load_3d(ring + st * L::Tile + d * L::Sub + i * box_rows * 128, map, &full[st], d * 64, y, page);
@@ -616,9 +641,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           const int key = k0 + (lt + 128 * i) / PR;
           c[i] = make_uint4(0, 0, 0, 0);
           if (key < p.hi) {
-            const int page = page_of(a.b, s, key);
+            const int page = page_of(a.b, p.seq, key);
             if (page >= 0) {
-              const long long kr = (((long long)page * a.heads + head) << shift) + (key & (page_rows - 1));
+              const long long kr = (((long long)page * a.heads + p.head) << shift) + (key & (page_rows - 1));
               c[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + kr * DIM + ((lt + 128 * i) % PR) * 16);
             }
           }
@@ -627,8 +652,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto hold_exp = [&](int j, const uint8_t* exps) -> uint32_t {
         const int key = p.lo + j * kManyKeys + lt;
         if (key >= p.hi) return 127u;
-        const int page = page_of(a.b, s, key);
-        return page < 0 ? 127u : exps[(((long long)page * a.heads + head) << shift) + (key & (page_rows - 1))];
+        const int page = page_of(a.b, p.seq, key);
+        return page < 0 ? 127u : exps[(((long long)page * a.heads + p.head) << shift) + (key & (page_rows - 1))];
       };
       auto put = [&](const uint4 (&c)[PT], uint8_t* to) {
 #pragma unroll
@@ -668,8 +693,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto q_src = [&](int i) {
         const int r = (i / CH) & 127, in = div_by(r, a.group, a.group_mul);
         const int tok = min((i / CH >> 7) * a.half_tokens + in, p.toks - 1);  // rows of no token: any
-        return static_cast<const T*>(a.q) + (long long)(q.tok0 + p.tok0 + tok) * a.q_token +
-               (long long)(head * a.group + r - in * a.group) * a.q_head + (i % CH) * 8;
+        return static_cast<const T*>(a.q) + (long long)(p.seq_tok0 + p.tok0 + tok) * a.q_token +
+               (long long)(p.head * a.group + r - in * a.group) * a.q_head + (i % CH) * 8;
       };
       auto q_dst = [&](int i) {
         const int r = i / CH, ch = i % CH;
@@ -764,7 +789,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           const int key = p.lo + j * kManyKeys + lt;
           uint8_t* vr = sv + st * L::Tile + lt * 128;
           bool odd = false;
-          if (key < q.len && key < p.hi) {
+          if (key < p.len && key < p.hi) {
 #pragma unroll
             for (int d = 0; d < DIM / 64; ++d)
 #pragma unroll 4
@@ -773,7 +798,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 odd |= not_finite2<M>(w.x) | not_finite2<M>(w.y) | not_finite2<M>(w.z) | not_finite2<M>(w.w);
               }
           }
-          if (odd || key >= q.len || key >= p.hi) {
+          if (odd || key >= p.len || key >= p.hi) {
 #pragma unroll
             for (int d = 0; d < DIM / 64; ++d)
 #pragma unroll 4
@@ -814,8 +839,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         tc_commit(&bar.sfull[t][h]);
       };
-      for (; more && ok; advance()) {
-        const ManyPart p = part();
+      while (ok && next_part()) {
+        part_read();
         if (p.j0 >= p.j1) continue;
         const int ja = t ? p.a[1] : p.a[0], jb = t ? p.b[1] : p.b[0];
         ok = many_wait1(&bar.qfull, np & 1, 1) && many_wait1(&bar.kfull[nb & 1], (nb >> 1) & 1, 1);
@@ -866,6 +891,31 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         many_wait1(&bar.kempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
         many_wait1(&bar.qempty, (np - 1) & 1, 3);
         many_wait1(&bar.vempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
+      }
+    }
+    if (warp == 15 && lane == 0) {
+      // ------------------------------------------------------------ parts
+      long long at = sc.cut[0].start, first = sc.cut[0].first;
+      const long long end = sc.cut[1].start;
+      int s = sc.cut[0].seq, head = sc.cut[0].head, tile = sc.cut[0].tile;
+      bool more = at < end, ok = true;
+      PagedSeq q = {};
+      if (more) q = paged_seq(a, s);
+      for (uint32_t n = 0; ok; ++n) {
+        ManyPart next;
+        next.live = 0;
+        if (more) {
+          const int units = paged_blocks<kManyKeys>(a, q, tile);
+          next = many_part(a, q, s, head, tile, paged_block_at(a, at, first, units), paged_block_at(a, end, first, units), units);
+          first += units + a.extra;
+          at = first;
+        }
+        if (n >= 2) ok = many_wait1(&bar.heard[n & 1], ((n >> 1) & 1) ^ 1, 2);
+        if (!ok) break;
+        parts[n & 1] = next;
+        mbar_arrive(&bar.told[n & 1]);
+        if (!more) break;
+        more = at < end && paged_next(a, &q, &s, &head, &tile);
       }
     }
     __syncwarp();
