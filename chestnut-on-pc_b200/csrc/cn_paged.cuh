@@ -102,7 +102,7 @@ __device__ __forceinline__ int paged_block_at(const PagedArgs& a, long long at, 
   return (int)min(max(at - first - a.extra, 0ll), (long long)n);
 }
 
-// Sum over the block; `scratch` has a long long for each warp.
+// Exclusive scan over the block and its total; `scratch` has a long long for each warp.
 template <int THREADS>
 __device__ __forceinline__ long long block_scan(long long v, long long* scratch, long long* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -114,15 +114,17 @@ __device__ __forceinline__ long long block_scan(long long v, long long* scratch,
   }
   if (lane == 31) scratch[warp] = x;
   __syncthreads();
-  long long before = 0, all = 0;
+  // each warp adds up the warps' sums with its lanes
+  long long y = lane < THREADS / 32 ? scratch[lane] : 0;
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += scratch[w];
-    all += scratch[w];
+  for (int o = 1; o < THREADS / 32; o <<= 1) {
+    const long long z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
   }
+  *total = __shfl_sync(0xffffffffu, y, THREADS / 32 - 1);
+  const long long before = __shfl_sync(0xffffffffu, y, max(warp - 1, 0));
   __syncthreads();
-  *total = all;
-  return before + x - v;  // exclusive
+  return (warp ? before : 0) + x - v;  // exclusive
 }
 
 // What a block needs to find its stretch (shared memory).
@@ -134,33 +136,34 @@ struct PagedScratch {
   PagedCut cut[2];
 };
 
-// Units of one head of sequences s0 .. s0 + THREADS - 1 into sc->seq_units.  A
-// warp takes a sequence and its lanes the tiles, a thread where a sequence has
-// one tile at most.
+// Units of one head of sequence s0 + (this thread), 0 behind the last.  A warp
+// takes a sequence and its lanes the tiles, a thread where a sequence has one
+// tile at most.
 template <int KEYS, int THREADS>
-__device__ __forceinline__ void paged_count(const PagedArgs& a, int s0, PagedScratch<THREADS>* sc) {
+__device__ __forceinline__ int paged_count(const PagedArgs& a, int s0, PagedScratch<THREADS>* sc) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int n = min(a.b.n_seqs - s0, THREADS);
   if (a.rows_max <= a.tile_tokens * a.group) {
+    if (tid >= n) return 0;
+    const PagedSeq q = paged_seq(a, s0 + tid);
+    return q.tiles ? paged_units<KEYS>(a, q, 0) : 0;
+  }
+  for (int i = tid >> 5; i < n; i += THREADS / 32) {
+    const PagedSeq q = paged_seq(a, s0 + i);
     int w = 0;
-    if (tid < n) {
-      const PagedSeq q = paged_seq(a, s0 + tid);
-      if (q.tiles) w = paged_units<KEYS>(a, q, 0);
-    }
-    sc->seq_units[tid] = w;
-  } else {
-    for (int i = tid >> 5; i < THREADS; i += THREADS / 32) {
-      int w = 0;
-      if (i < n) {
-        const PagedSeq q = paged_seq(a, s0 + i);
-        for (int b = lane; b < q.tiles; b += 32) w += paged_units<KEYS>(a, q, b);
+    for (int b = lane; b < q.tiles; b += 32) w += paged_units<KEYS>(a, q, b);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-      }
-      if (lane == 0) sc->seq_units[i] = w;
-    }
+    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+    if (lane == 0) sc->seq_units[i] = w;
   }
   __syncthreads();
+  return tid < n ? sc->seq_units[tid] : 0;
+}
+
+// total * c / n (64-bit divisions take about as long as all the rest here).
+__device__ __forceinline__ long long paged_share(long long total, int c, int n) {
+  if (total < (1ll << 22)) return (uint32_t)total * (uint32_t)c / (uint32_t)n;
+  return total * c / n;
 }
 
 // The stretch of CTA `c`: sc->cut[0] where it begins, sc->cut[1] where it ends,
@@ -168,16 +171,19 @@ __device__ __forceinline__ void paged_count(const PagedArgs& a, int s0, PagedScr
 template <int KEYS, int THREADS>
 __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScratch<THREADS>* sc) {
   const int tid = threadIdx.x, lane = tid & 31;
-  long long total = 0;
+  long long total = 0, before = 0, at = 0;
+  int each = 0;
   for (int s0 = 0; s0 < a.b.n_seqs; s0 += THREADS) {
     long long all;
-    paged_count<KEYS, THREADS>(a, s0, sc);
-    block_scan<THREADS>((long long)a.heads * sc->seq_units[tid], sc->warp_sum, &all);
+    each = paged_count<KEYS, THREADS>(a, s0, sc);
+    at = block_scan<THREADS>((long long)a.heads * each, sc->warp_sum, &all);
     total += all;
   }
   // CTAs that take part: each has min_units units or more
-  const long long ctas = min((long long)a.ctas, max((total + a.min_units - 1) / a.min_units, 1ll));
-  const long long u[2] = {c < ctas ? total * c / ctas : total, c + 1 < ctas ? total * (c + 1) / ctas : total};
+  int ctas = a.ctas;
+  if (total < (long long)a.ctas * a.min_units) ctas = max(((int)total + a.min_units - 1) / a.min_units, 1);
+  const long long u[2] = {c < ctas ? paged_share(total, c, ctas) : total,
+                          c + 1 < ctas ? paged_share(total, c + 1, ctas) : total};
   if (tid < 2) {
     PagedCut& k = sc->cut[tid];
     k.start = k.first = k.total = total;
@@ -185,29 +191,30 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
     k.head = k.tile = k.units = 0;
   }
   __syncthreads();
-  long long before = 0;
   for (int s0 = 0; s0 < a.b.n_seqs; s0 += THREADS) {
-    if (a.b.n_seqs > THREADS) paged_count<KEYS, THREADS>(a, s0, sc);  // else it lies there still
-    const long long w = (long long)a.heads * sc->seq_units[tid];
-    long long all;
-    const long long at = before + block_scan<THREADS>(w, sc->warp_sum, &all);
+    if (a.b.n_seqs > THREADS) {  // else the only pass's results are still at hand
+      long long all;
+      each = paged_count<KEYS, THREADS>(a, s0, sc);
+      at = before + block_scan<THREADS>((long long)a.heads * each, sc->warp_sum, &all);
+      before += all;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (u[i] >= at && u[i] < at + w) {  // the sequence's thread
+      if (u[i] >= at && u[i] < at + (long long)a.heads * each) {  // the sequence's thread
         sc->cut[i].seq = s0 + tid;
         sc->seq_at[i] = at;
-        sc->seq_each[i] = sc->seq_units[tid];
+        sc->seq_each[i] = each;
       }
-    before += all;
-    __syncthreads();  // seq_units is read by everyone before it is counted anew
   }
+  __syncthreads();
   if (tid < 64) {  // a warp for each end: the tile of its sequence
     PagedCut& k = sc->cut[tid >> 5];
     if (k.seq >= 0) {
       const PagedSeq q = paged_seq(a, k.seq);
-      const long long rel = u[tid >> 5] - sc->seq_at[tid >> 5], each = sc->seq_each[tid >> 5];
-      const int head = (int)(rel / each);
-      const int in_head = (int)(rel - head * each);
+      const long long rel = u[tid >> 5] - sc->seq_at[tid >> 5];
+      const int each1 = (int)sc->seq_each[tid >> 5];
+      const int head = rel < (1ll << 31) ? (int)((uint32_t)rel / (uint32_t)each1) : (int)(rel / each1);
+      const int in_head = (int)(rel - (long long)head * each1);
       int begin = 0;  // units of the head before tile b0
       for (int b0 = 0; b0 < q.tiles; b0 += 32) {
         const int n = b0 + lane < q.tiles ? paged_units<KEYS>(a, q, b0 + lane) : 0;
@@ -221,7 +228,7 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
         if (here) {
           k.head = head;
           k.tile = b0 + lane;
-          k.first = sc->seq_at[tid >> 5] + head * each + begin + x - n;
+          k.first = sc->seq_at[tid >> 5] + (long long)head * each1 + begin + x - n;
           k.units = n;
           k.start = n - a.extra <= a.snap || u[tid >> 5] - k.first <= a.extra ? k.first : u[tid >> 5];
         }

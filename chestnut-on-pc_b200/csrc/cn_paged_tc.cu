@@ -125,7 +125,7 @@ __device__ __forceinline__ bool many_edge(const ManyPart& p, int j) {
 // takes about as long to read as a whole block's products).
 constexpr long long kManyWaitClocks = 4000000000ll;  // ~2 s
 __device__ __forceinline__ bool many_wait1(uint64_t* bar, uint32_t parity, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (__builtin_expect(mbar_try_wait(bar, parity), 1)) return true;
   const long long t0 = clock64();
   while (!mbar_try_wait(bar, parity))
     if (clock64() - t0 > kManyWaitClocks) {
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           tc_fence_after();
           const uint32_t th = ts + h * 64;
           const int k0 = p.lo + j * kManyKeys + h * 64;
-          if (edge) {
+          if (__builtin_expect(edge, 0)) {
             if (h == 0) {  // its V is in order, and what lies beside it
               ok = many_wait(&bar.vfix[st], fix, 2);
               if (!ok) break;
@@ -457,12 +457,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           const uint32_t odd = edge ? bad[st][2 * h] | bad[st][2 * h + 1] : 0u;
           const bool begun = j > ja || h > 0;  // there are sums in O
           const bool any = __any_sync(0xffffffffu, raise);
-          if (begun && (any || odd)) {  // O stands still once the product before this one is added
+          if (__builtin_expect(begun && (any || odd), 0)) {  // O stands still once the product before this one is added
             ok = many_wait(&bar.odone[t][h ^ 1], (ns + h + 1) & 1, 3);
             if (!ok) break;
             tc_fence_after();
           }
-          if (any) {
+          if (__builtin_expect(any, 0)) {
             const float c = raise ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
             if (raise) m = top;
             l *= c;
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
           }
           const float sub = m == -INFINITY ? 0.f : -m;
-          if (odd) {
+          if (__builtin_expect(odd, 0)) {
             // rows of V that are not finite: for the rows that see them, from the cache itself
             tmem_st_wait();
 #pragma unroll 1
