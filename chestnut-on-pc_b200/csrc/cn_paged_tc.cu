@@ -28,6 +28,7 @@
 // see them, leave the product and are added by the threads whose row sees them.
 // An 8-bit cache's powers of two: see cn_paged.cu; the loaders leave them as
 // (2^ek * scale, ev, 2^-ev) of each key.
+#include <type_traits>
 #include "cn_paged.cuh"
 
 namespace cn {
@@ -72,7 +73,8 @@ struct ManyPart {
   int lo;          // position of the tile's unit 0
   int j0, j1;      // blocks of 128 keys, from lo
   int a[2], b[2];  // those that the halves take part in
-  int all_lo, all_hi, hi;
+  int hi;          // keys behind it no row sees
+  int i0, i1;      // blocks that every row sees whole; the others are at the edge
   int tok0, toks;  // tokens of the sequence
   int seq, head, seq_tok0, past, len;
   int whole, first_part;  // the whole tile; its beginning
@@ -110,15 +112,16 @@ __device__ __forceinline__ ManyPart many_part(const PagedArgs& a, const PagedSeq
     }
   }
   const int first_pos = q.past + p.tok0, last_pos = first_pos + p.toks - 1;
-  p.all_hi = first_pos < 0 ? 0 : a.causal ? min(q.len, first_pos + 1) : q.len;
-  p.all_lo = a.window > 0 ? last_pos - a.window + 1 : 0;
+  const int all_hi = first_pos < 0 ? 0 : a.causal ? min(q.len, first_pos + 1) : q.len;
+  const int all_lo = a.window > 0 ? max(last_pos - a.window + 1, 0) : 0;
+  p.i0 = max(all_lo - p.lo + kManyKeys - 1, 0) / kManyKeys;
+  p.i1 = max(all_hi - p.lo, 0) / kManyKeys;
   return p;
 }
 
 // Whether some row of the tile does not see all of block j.
 __device__ __forceinline__ bool many_edge(const ManyPart& p, int j) {
-  const int k0 = p.lo + j * kManyKeys;
-  return k0 < p.all_lo || k0 + kManyKeys > p.all_hi;
+  return j < p.i0 || j >= p.i1;
 }
 
 // Bounded wait on the critical path: the limit goes by the SM's clock (%globaltimer
@@ -375,46 +378,38 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tmem_st_wait();
       }
       float rs = 1.f;
-#pragma unroll 1
-      for (int j = p.j0; j < p.j1 && ok; ++j) {
+      // 64 keys of block j; EDGE: some row of the tile does not see all of the block.  Two copies of
+      // the code: what edges need, between the lines of the common path, slows it by a tenth.
+      auto step = [&](auto edge_block, int j, int h) {
+        constexpr bool EDGE = decltype(edge_block)::value;
         const uint32_t n = nb + j - p.j0, st = n & 1;
-        const bool edge = many_edge(p, j);
-        const uint32_t fix = (fixes >> st) & 1;
-        if (edge) fixes ^= 1u << st;
-        if (j < ja || j >= jb) continue;
+        if (!many_wait(&bar.sfull[t][h], ns & 1, 3)) return false;
+        tc_fence_after();
+        const uint32_t th = ts + h * 64;
+        if constexpr (EDGE) {
+          if (h == 0) {  // its V is in order, and what lies beside it
+            if (!many_wait(&bar.vfix[st], (fixes >> st) & 1, 2)) return false;
+          }
+          // what a row does not see becomes -inf in tensor memory; all else goes on as everywhere
+          const int k0 = p.lo + j * kManyKeys + h * 64, clo = see_lo - k0, chi = see_hi - k0;
 #pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
-          ok = many_wait(&bar.sfull[t][h], ns & 1, 3);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t th = ts + h * 64;
-          const int k0 = p.lo + j * kManyKeys + h * 64;
-          if (__builtin_expect(edge, 0)) {
-            if (h == 0) {  // its V is in order, and what lies beside it
-              ok = many_wait(&bar.vfix[st], fix, 2);
-              if (!ok) break;
-            }
-            // what a row does not see becomes -inf in tensor memory; all else goes on as everywhere
-            const int clo = see_lo - k0, chi = see_hi - k0;
-#pragma unroll 1
-            for (int c0 = 0; c0 < 64; c0 += 32) {
-              uint32_t y[32];
-              tmem_ld32(th + c0, y);
-              tmem_ld_wait32(y);
+          for (int c0 = 0; c0 < 64; c0 += 32) {
+            uint32_t y[32];
+            tmem_ld32(th + c0, y);
+            tmem_ld_wait32(y);
 #pragma unroll
-              for (int c = 0; c < 32; ++c)
-                if (c0 + c < clo || c0 + c >= chi) y[c] = 0xff800000u;
-              tmem_st32(th + c0, y);
-            }
-            tmem_st_wait();
+            for (int c = 0; c < 32; ++c)
+              if (c0 + c < clo || c0 + c >= chi) y[c] = 0xff800000u;
+            tmem_st32(th + c0, y);
           }
-          if constexpr (CODED) {
-            if (h == 0) {
-              if constexpr (std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][t * 128 + r];
-              ok = many_wait(&bar.vfull[st], (n >> 1) & 1, 1);
-              if (!ok) break;
-            }
+          tmem_st_wait();
+        }
+        if constexpr (CODED) {
+          if (h == 0) {
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][t * 128 + r];
+            if (!many_wait(&bar.vfull[st], (n >> 1) & 1, 1)) return false;
           }
+        }
           uint32_t s0[32], s1[32];
           tmem_ld32(th, s0);
           tmem_ld32(th + 32, s1);
@@ -454,12 +449,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           if constexpr (!CODED) top *= a.scale;
           const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
-          const uint32_t odd = edge ? bad[st][2 * h] | bad[st][2 * h + 1] : 0u;
+          const uint32_t odd = EDGE ? bad[st][2 * h] | bad[st][2 * h + 1] : 0u;
           const bool begun = j > ja || h > 0;  // there are sums in O
           const bool any = __any_sync(0xffffffffu, raise);
           if (__builtin_expect(begun && (any || odd), 0)) {  // O stands still once the product before this one is added
-            ok = many_wait(&bar.odone[t][h ^ 1], (ns + h + 1) & 1, 3);
-            if (!ok) break;
+            if (!many_wait(&bar.odone[t][h ^ 1], (ns + h + 1) & 1, 3)) return false;
             tc_fence_after();
           }
           if (__builtin_expect(any, 0)) {
@@ -479,7 +473,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
           }
           const float sub = m == -INFINITY ? 0.f : -m;
-          if (__builtin_expect(odd, 0)) {
+          if (EDGE && odd) {
             // rows of V that are not finite: for the rows that see them, from the cache itself
             tmem_st_wait();
 #pragma unroll 1
@@ -490,7 +484,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 w = exp2_approx(fmaf(w * rs, kvx[st][(h * 64 + c) >> 1][0][c & 1], kvx[st][(h * 64 + c) >> 1][1][c & 1]) + sub);
               else
                 w = exp2_approx(fmaf(w, a.scale, sub));
-              const int key = k0 + c;
+              const int key = p.lo + j * kManyKeys + h * 64 + c;
               const bool see = key >= see_lo && key < see_hi;
               const int page = page_of(a.b, p.seq, key);
               const long long vr = (((long long)max(page, 0) * a.heads + p.head) << a.b.page_shift) + (key & ((1 << a.b.page_shift) - 1));
@@ -553,8 +547,28 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(&bar.pfull[t][h]);
+        return true;
+      };
+      // blocks [i0, i1) are not at the edge
+      const int i0 = min(max(p.i0, ja), jb), i1 = min(max(p.i1, i0), jb);
+#pragma unroll 1
+      for (int j = p.j0; j < p.j1 && ok; ++j) {
+        if (j < i0 || j >= i1) {
+          if (j >= ja && j < jb) {
+#pragma unroll 1
+            for (int h = 0; h < 2 && ok; ++h) ok = step(std::true_type(), j, h);
+            ++ns;
+          }
+          if (j < p.i0 || j >= p.i1) fixes ^= 1u << ((nb + j - p.j0) & 1);
+          continue;
         }
-        ++ns;
+#pragma unroll 1
+        for (; j < i1 && ok; ++j) {
+#pragma unroll 1
+          for (int h = 0; h < 2 && ok; ++h) ok = step(std::false_type(), j, h);
+          ++ns;
+        }
+        --j;
       }
       nb += p.j1 - p.j0;
       np += p.j1 > p.j0;
