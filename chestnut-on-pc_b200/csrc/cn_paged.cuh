@@ -38,6 +38,7 @@ struct PagedArgs {
   struct PagedCut* cuts;   // [ctas + 1]
   float* part_o;           // [2 * ctas][ROWS][DIM]
   float* part_ml;          // [2 * ctas][ROWS][2]
+  float* part_x;           // tcgen05 kernel: [ctas][2][2][128][DIM / 2], between the halves of a dual part
 };
 
 // Where CTA c's stretch begins: unit `start` of the line, inside tile (seq,

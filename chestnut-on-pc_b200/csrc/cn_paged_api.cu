@@ -8,13 +8,14 @@ namespace {
 
 // Workspace of one launch: the cuts, then the parts.
 struct PagedSpace {
-  size_t o, ml, bytes;
+  size_t o, ml, x, bytes;
 };
 PagedSpace paged_space(int ctas, int rows, int dim) {
   PagedSpace s;
   s.o = ((size_t)(ctas + 1) * sizeof(PagedCut) + 255) / 256 * 256;
   s.ml = s.o + (size_t)2 * ctas * rows * dim * 4;
-  s.bytes = s.ml + ((size_t)2 * ctas * rows * 2 * 4 + 255) / 256 * 256;
+  s.x = s.ml + ((size_t)2 * ctas * rows * 2 * 4 + 255) / 256 * 256;
+  s.bytes = s.x + (rows == kManyRows ? (size_t)ctas * 4 * 128 * (dim / 2) * 4 : 0);
   return s;
 }
 
@@ -233,6 +234,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     m.cuts = reinterpret_cast<PagedCut*>(w);
     m.part_o = reinterpret_cast<float*>(w + many.o);
     m.part_ml = reinterpret_cast<float*>(w + many.ml);
+    m.part_x = reinterpret_cast<float*>(w + many.x);
     c.merge_many = cap > (long long)m.snap * kManyKeys;
     if (!coded && (paged_map(&c.tk, cache, cache->k) || paged_map(&c.tv, cache, cache->v))) return CN_ERR_CUDA;
   }

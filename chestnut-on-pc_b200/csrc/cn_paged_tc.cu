@@ -54,17 +54,19 @@ struct Many {
   static constexpr int Sub = 128 * 128;            // 128 rows x 64 values of 16 bits
   static constexpr int Tile = DIM / 64 * Sub;      // 128 rows
   static constexpr int QBytes = 2 * Tile;
-  static constexpr int Stages = 2;                 // of K, and of V
+  static constexpr int Stages = DIM == 128 ? 2 : 4;  // of K, and of V; even: see ManyPart::dual
   static constexpr size_t Smem = 1024 + QBytes + 2 * Stages * Tile;
 };
 
 struct ManyBars {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], vfix[2];  // stages
+  uint64_t kfull[4], kempty[4], vfull[4], vempty[4], vfix[4];  // stages
   uint64_t sfull[2][2], pfull[2][2];                           // [half][64 keys of a block]
   uint64_t odone[2][2];                                        // its product with V is added to O
   uint64_t asked;                                              // V of an edge block is on its way
   uint64_t qfull, qempty;
   uint64_t told[2], heard[2];                                  // parts: worked out, read by all
+  uint64_t joined;                                             // both halves' sums of a dual part are out
+  uint64_t drain[2];
   uint32_t tmem;
 };
 
@@ -78,6 +80,7 @@ struct ManyPart {
   int tok0, toks;  // tokens of the sequence
   int seq, head, seq_tok0, past, len;
   int whole, first_part;  // the whole tile; its beginning
+  int dual;               // the tile's tokens fill one half at most: the other one takes every second block of keys
   int live;               // 0: no further part
 };
 
@@ -110,6 +113,11 @@ __device__ __forceinline__ ManyPart many_part(const PagedArgs& a, const PagedSeq
         if (p.b[t] < p.a[t]) p.a[t] = p.b[t] = p.j1;
       }
     }
+  }
+  p.dual = p.toks <= a.half_tokens && p.b[0] - p.a[0] >= 2;
+  if (p.dual) {
+    p.a[1] = p.a[0];
+    p.b[1] = p.b[0];
   }
   const int first_pos = q.past + p.tok0, last_pos = first_pos + p.toks - 1;
   const int all_hi = first_pos < 0 ? 0 : a.causal ? min(q.len, first_pos + 1) : q.len;
@@ -291,29 +299,33 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __shared__ PagedScratch<kManyThreads> sc;
   __shared__ ManyBars bar;
   __shared__ ManyPart parts[2];
-  __shared__ uint32_t bad[2][4];                        // V rows of an edge block that are not finite
+  __shared__ float2 join_ml[2][2][128];                 // (m, l) of a dual part's halves (such parts in turn)
+  __shared__ uint32_t bad[L::Stages][4];                        // V rows of an edge block that are not finite
   // 8-bit cache, of each pair of keys: {scale 2^ek, scale 2^ek'}, {ev, ev'}; and {2^-ev, 2^-ev'}
-  __shared__ __align__(16) float kvx[CODED ? 2 : 1][CODED ? 64 : 1][2][2];
-  __shared__ __align__(16) float vback[CODED ? 2 : 1][CODED ? 64 : 1][2];
+  __shared__ __align__(16) float kvx[CODED ? L::Stages : 1][CODED ? 64 : 1][2][2];
+  __shared__ __align__(16) float vback[CODED ? L::Stages : 1][CODED ? 64 : 1][2];
   __shared__ float qpow[2][CODED ? kManyRows : 1];      // power of two that a row of Q was divided by (parts in turn)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < L::Stages; ++i) {
       mbar_init(&bar.kfull[i], CODED ? 128 : 1);
       mbar_init(&bar.vfull[i], CODED ? 128 : 1);
       mbar_init(&bar.kempty[i], 2);
       mbar_init(&bar.vempty[i], 2);
       mbar_init(&bar.vfix[i], 128);
-      mbar_init(&bar.sfull[i][0], 1);
-      mbar_init(&bar.sfull[i][1], 1);
-      mbar_init(&bar.pfull[i][0], 128);
-      mbar_init(&bar.pfull[i][1], 128);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.drain[i], 1);
       mbar_init(&bar.told[i], 1);
       mbar_init(&bar.heard[i], 14);  // 8 softmax warps, 4 of the loads, 2 of the products
-      mbar_init(&bar.odone[i][0], 1);
-      mbar_init(&bar.odone[i][1], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bar.sfull[i][h], 1);
+        mbar_init(&bar.pfull[i][h], 128);
+        mbar_init(&bar.odone[i][h], 1);
+      }
     }
+    mbar_init(&bar.joined, 256);
     mbar_init(&bar.qfull, 128);
     mbar_init(&bar.qempty, 2);
     mbar_init(&bar.asked, 1);
@@ -356,13 +368,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
     // so far: blocks of this half, blocks and parts of the CTA; fixes: phase bit of a stage
-    uint32_t ns = 0, nb = 0, np = 0, fixes = 0;
+    uint32_t ns = 0, nb = 0, np = 0, fixes = 0, duals = 0;
     bool ok = true;
     while (ok) {
       if (!__all_sync(0xffffffffu, next_part())) break;
       __syncwarp();
       if (lane == 0) part_read();
-      const int tok = t * a.half_tokens + my_i;  // of the tile
+      const int tok = (p.dual ? 0 : t * a.half_tokens) + my_i;  // of the tile
       const bool live = my_i < a.half_tokens && tok < p.toks;
       const int pos = live ? p.past + p.tok0 + tok : -1;
       const int see_hi = pos < 0 ? 0 : a.causal ? min(p.len, pos + 1) : p.len;
@@ -378,11 +390,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tmem_st_wait();
       }
       float rs = 1.f;
+      const uint32_t ns0 = ns;
       // 64 keys of block j; EDGE: some row of the tile does not see all of the block.  Two copies of
       // the code: what edges need, between the lines of the common path, slows it by a tenth.
       auto step = [&](auto edge_block, int j, int h) {
         constexpr bool EDGE = decltype(edge_block)::value;
-        const uint32_t n = nb + j - p.j0, st = n & 1;
+        const uint32_t n = nb + j - p.j0, st = n % L::Stages;
         if (!many_wait(&bar.sfull[t][h], ns & 1, 3)) return false;
         tc_fence_after();
         const uint32_t th = ts + h * 64;
@@ -406,8 +419,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         if constexpr (CODED) {
           if (h == 0) {
-            if constexpr (std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][t * 128 + r];
-            if (!many_wait(&bar.vfull[st], (n >> 1) & 1, 1)) return false;
+            if constexpr (std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][(p.dual ? 0 : t * 128) + r];
+            if (!many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1)) return false;
           }
         }
           uint32_t s0[32], s1[32];
@@ -450,7 +463,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           if constexpr (!CODED) top *= a.scale;
           const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
           const uint32_t odd = EDGE ? bad[st][2 * h] | bad[st][2 * h + 1] : 0u;
-          const bool begun = j > ja || h > 0;  // there are sums in O
+          const bool begun = ns > ns0 || h > 0;  // there are sums in O
           const bool any = __any_sync(0xffffffffu, raise);
           if (__builtin_expect(begun && (any || odd), 0)) {  // O stands still once the product before this one is added
             if (!many_wait(&bar.odone[t][h ^ 1], (ns + h + 1) & 1, 3)) return false;
@@ -549,21 +562,24 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           mbar_arrive(&bar.pfull[t][h]);
         return true;
       };
+      // a dual part's blocks by their stages: even ones are half 0's
+      auto own = [&](int j) { return j >= ja && j < jb && (!p.dual || ((nb + j - p.j0) & 1) == t); };
       // blocks [i0, i1) are not at the edge
       const int i0 = min(max(p.i0, ja), jb), i1 = min(max(p.i1, i0), jb);
 #pragma unroll 1
       for (int j = p.j0; j < p.j1 && ok; ++j) {
         if (j < i0 || j >= i1) {
-          if (j >= ja && j < jb) {
+          if (own(j)) {
 #pragma unroll 1
             for (int h = 0; h < 2 && ok; ++h) ok = step(std::true_type(), j, h);
             ++ns;
           }
-          if (j < p.i0 || j >= p.i1) fixes ^= 1u << ((nb + j - p.j0) & 1);
+          if (many_edge(p, j)) fixes ^= 1u << ((nb + j - p.j0) % L::Stages);
           continue;
         }
 #pragma unroll 1
         for (; j < i1 && ok; ++j) {
+          if (!own(j)) continue;
 #pragma unroll 1
           for (int h = 0; h < 2 && ok; ++h) ok = step(std::false_type(), j, h);
           ++ns;
@@ -580,13 +596,43 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if (!ok) break;
         tc_fence_after();
       }
+      int d0 = 0, d1 = DIM;  // the columns that this half writes out
+      float c = 1.f, c2 = 0.f;
+      const float* theirs = nullptr;
+      if (p.dual) {
+        // Each half hands the other one its sums of the other one's columns (through L2: the
+        // rings are full already of the next part) and joins its own.
+        float* mine = a.part_x + (((long long)blockIdx.x * 2 + (duals & 1)) * 2 + t) * 128 * (DIM / 2) + (long long)r * (DIM / 2);
+#pragma unroll 1
+        for (int d = 0; d < DIM / 2; d += 32) {
+          uint32_t o[32];
+          tmem_ld32(to + (t ^ 1) * (DIM / 2) + d, o);
+          tmem_ld_wait32(o);
+          st_row64(mine + d, o, true);
+          st_row64(mine + d + 16, o + 16, true);
+        }
+        join_ml[duals & 1][t][r] = make_float2(m, l);
+        mbar_arrive(&bar.joined);
+        ok = many_wait(&bar.joined, duals & 1, 3);
+        if (!ok) break;
+        const float2 ml = join_ml[duals & 1][t ^ 1][r];
+        theirs = a.part_x + (((long long)blockIdx.x * 2 + (duals & 1)) * 2 + (t ^ 1)) * 128 * (DIM / 2) + (long long)r * (DIM / 2);
+        ++duals;
+        const float top = fmaxf(m, ml.x);
+        c = m == -INFINITY ? 0.f : exp2_approx(m - top);
+        c2 = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - top);
+        l = l * c + ml.y * c2;
+        m = top;
+        d0 = t * (DIM / 2);
+        d1 = d0 + DIM / 2;
+      }
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       T* out = static_cast<T*>(a.out) + (long long)(p.seq_tok0 + p.tok0 + tok) * a.o_token +
                (long long)(p.head * a.group + my_h) * a.o_head;
-      const long long pr = slot * kManyRows + t * 128 + r;
+      const long long pr = slot * kManyRows + (p.dual ? 0 : t * 128) + r;
       const bool wide = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
 #pragma unroll 1
-      for (int d = 0; d < DIM; d += 32) {
+      for (int d = d0; d < d1; d += 32) {
         uint32_t o[32];
         if (ja < jb) {
           tmem_ld32(to + d, o);
@@ -594,6 +640,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (p.dual) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(theirs + d - d0 + i));
+            o[i] = __float_as_uint(fmaf(x.x, c2, __uint_as_float(o[i]) * c));
+            o[i + 1] = __float_as_uint(fmaf(x.y, c2, __uint_as_float(o[i + 1]) * c));
+            o[i + 2] = __float_as_uint(fmaf(x.z, c2, __uint_as_float(o[i + 2]) * c));
+            o[i + 3] = __float_as_uint(fmaf(x.w, c2, __uint_as_float(o[i + 3]) * c));
+          }
         }
         if (live) {
           if (p.whole) {
@@ -608,7 +664,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
         }
       }
-      if (live && !p.whole) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(m, l);
+      if (live && !p.whole && d0 == 0) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(m, l);
       tc_fence_before();  // the next part's zeros and products come after these loads
     }
   } else if (warp < 12) {
@@ -626,22 +682,25 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       if (p.j0 >= p.j1) continue;
       const int blocks = p.j1 - p.j0;
 
-      // 16-bit cache: thread 0 asks for block j of K or V
-      auto fetch = [&](int j, uint32_t n, const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty) {
-        const uint32_t st = n & 1;
-        if (n >= 2 && !many_wait1(&empty[st], ((n >> 1) & 1) ^ 1, 2)) return false;
+      // 16-bit cache: a warp asks for the blocks of K and another one for those of V (whose stages
+      // come free later: one warp for both held K back), a lane for a page.  The pages of a block are
+      // looked up while the one before it is on its way.
+      auto look_up = [&](int j) {
         const int k0 = p.lo + j * kManyKeys;
         const int boxes = (min(kManyKeys, p.hi - k0) + box_rows - 1) / box_rows;
-        uint32_t bytes = 0;
-        for (int i = 0; i < boxes; ++i) bytes += page_of(a.b, p.seq, k0 + i * box_rows) >= 0 ? box_rows * DIM * 2 : 0;
-        mbar_arrive_expect_tx(&full[st], bytes);
-        for (int i = 0; i < boxes; ++i) {
-          const int page = page_of(a.b, p.seq, k0 + i * box_rows);
-          if (page < 0) continue;
-          const int y = p.head * page_rows + ((k0 + i * box_rows) & (page_rows - 1));
+        return j < p.j1 && lane < boxes ? page_of(a.b, p.seq, k0 + lane * box_rows) : -1;
+      };
+      auto fetch = [&](int j, int page, uint32_t n, const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty) {
+        const uint32_t st = n % L::Stages;
+        if (n >= L::Stages && !many_wait(&empty[st], ((n / L::Stages) & 1) ^ 1, 2)) return false;
+        const uint32_t pages = __popc(__ballot_sync(0xffffffffu, page >= 0));
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], pages * box_rows * DIM * 2);
+        __syncwarp();
+        if (page >= 0) {
+          const int y = p.head * page_rows + ((p.lo + j * kManyKeys + lane * box_rows) & (page_rows - 1));
 #pragma unroll
           for (int d = 0; d < DIM / 64; ++d)
-            tma_load_3d(ring + st * L::Tile + d * L::Sub + i * box_rows * 128, map, &full[st], d * 64, y, page);
+            tma_load_3d(ring + st * L::Tile + d * L::Sub + lane * box_rows * 128, map, &full[st], d * 64, y, page);
         }
         return true;
       };
@@ -689,14 +748,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 
       uint4 ck[PT], cv[PT];
       uint32_t ek = 0, ev = 0;
+      int page = -1;
       if constexpr (CODED) {
         hold(p.j0, a.k, ck);
         ek = hold_exp(p.j0, a.k_exp);
         hold(p.j0, a.v, cv);
         ev = hold_exp(p.j0, a.v_exp);
       } else {
-        if (lt == 0) ok = fetch(p.j0, nb, &tm_k, sk, bar.kfull, bar.kempty);
-        ok = __all_sync(0xffffffffu, ok);
+        if (warp == 8) {
+          ok = fetch(p.j0, look_up(p.j0), nb, &tm_k, sk, bar.kfull, bar.kempty);
+          page = look_up(p.j0 + 1);
+        } else if (warp == 9) {
+          page = look_up(p.j0);
+        }
       }
 
       // ---- Q: 128 or 256 rows, swizzled
@@ -756,14 +820,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // ---- blocks
       for (int i = 0; i < blocks && ok; ++i) {
         const int j = p.j0 + i;
-        const uint32_t n = nb + i, st = n & 1;
+        const uint32_t n = nb + i, st = n % L::Stages;
         const bool edge = many_edge(p, j);
         if constexpr (CODED) {
-          if (n >= 2) ok = many_wait(&bar.kempty[st], ((n >> 1) & 1) ^ 1, 2);
+          if (n >= L::Stages) ok = many_wait(&bar.kempty[st], ((n / L::Stages) & 1) ^ 1, 2);
           if (!ok) break;
           // kvx and vback of a stage are read by the softmax of its block, which is over when its
           // products with V are: kempty alone would not say so
-          if (n >= 2) ok = many_wait(&bar.vempty[st], ((n >> 1) & 1) ^ 1, 2);
+          if (n >= L::Stages) ok = many_wait(&bar.vempty[st], ((n / L::Stages) & 1) ^ 1, 2);
           if (!ok) break;
           put(ck, sk + st * L::Tile);
           kvx[st][lt >> 1][0][lt & 1] = exp_byte(ek) * a.scale;
@@ -783,22 +847,24 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             ev = hold_exp(j + 1, a.v_exp);
           }
         } else {
-          if (lt == 0) {
-            ok = fetch(j, n, &tm_v, sv, bar.vfull, bar.vempty);
-            if (ok && i + 1 < blocks) ok = fetch(j + 1, n + 1, &tm_k, sk, bar.kfull, bar.kempty);
+          if (warp == 8) {
+            if (i + 1 < blocks) ok = fetch(j + 1, page, n + 1, &tm_k, sk, bar.kfull, bar.kempty);
+            page = look_up(j + 2);
+          } else if (warp == 9) {
+            ok = fetch(j, page, n, &tm_v, sv, bar.vfull, bar.vempty);
+            page = look_up(j + 1);
           }
-          ok = __all_sync(0xffffffffu, ok);
         }
         if (edge && ok) {
-          // the other warps come here ahead of the thread that asks for the blocks: a parity says
+          // the other warps come here ahead of the one that asks for V: a parity says
           // nothing about a block that is not asked for yet
           if constexpr (!CODED) {
-            if (lt == 0) mbar_arrive(&bar.asked);
-            ok = many_wait(&bar.asked, edges & 1, 2);
+            if (lt == 32) mbar_arrive(&bar.asked);
+            ok = __all_sync(0xffffffffu, mbar_wait(&bar.asked, edges & 1, 2));  // asleep: three warps wait here long
             ++edges;
             if (!ok) break;
           }
-          ok = many_wait(&bar.vfull[st], (n >> 1) & 1, 1);
+          ok = many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1);
           if (!ok) break;
           const int key = p.lo + j * kManyKeys + lt;
           uint8_t* vr = sv + st * L::Tile + lt * 128;
@@ -827,7 +893,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
       nb += blocks;
     }
-    if (!ok && !CODED && lt == 0) {  // given up: the copies in flight land before the block ends
+    if (!ok && !CODED && lane == 0) {  // given up: the copies in flight land before the block ends
       const unsigned long long t0 = global_ns();
       while (global_ns() - t0 < 100000000ull) {
       }
@@ -840,10 +906,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const int t = warp - 12;
       uint32_t nb = 0, np = 0, ns = 0, fixes = 0;
       bool ok = true;
-      const uint32_t q_lo = desc_lo(sq + t * L::Tile, 16), k_lo = desc_lo(sk, 16), v_lo = desc_lo(sv, L::Sub);
+      const uint32_t q_lo0 = desc_lo(sq, 16), k_lo = desc_lo(sk, 16), v_lo = desc_lo(sv, L::Sub);
       const uint32_t d_s = tmem + t * 128, d_o = tmem + 256 + t * 128;
       // S of keys h * 64 .. of a block: rows h * 64 .. of the K tile
-      auto scores = [&](int h, uint32_t st) {
+      auto scores = [&](uint32_t q_lo, int h, uint32_t st) {
         const uint32_t ka = k_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4);
         tc_mma_ss<false>(d_s + h * 64, q_lo, ka, id_s);
 #pragma unroll
@@ -853,59 +919,110 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         tc_commit(&bar.sfull[t][h]);
       };
+      // O += P V of those keys
+      auto sums = [&](int h, uint32_t st) {
+        const uint32_t va = v_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc_mma_ts(d_o, d_s + h * 64 + k * 8, va + k * (2048 >> 4), id_o);
+        tc_commit(&bar.odone[t][h]);
+      };
+      auto stage = [](uint32_t n) { return n % L::Stages; };
+      auto phase = [](uint32_t n) { return (n / L::Stages) & 1; };
+      auto v_there = [&](int j, uint32_t n) {
+        if (!many_wait1(&bar.vfull[stage(n)], phase(n), 1)) return false;
+        return !many_edge(p, j) || many_wait1(&bar.vfix[stage(n)], (fixes >> stage(n)) & 1, 1);
+      };
       while (ok && next_part()) {
         part_read();
         if (p.j0 >= p.j1) continue;
         const int ja = t ? p.a[1] : p.a[0], jb = t ? p.b[1] : p.b[0];
-        ok = many_wait1(&bar.qfull, np & 1, 1) && many_wait1(&bar.kfull[nb & 1], (nb >> 1) & 1, 1);
+        const uint32_t q_lo = q_lo0 + (p.dual ? 0 : t * (L::Tile >> 4));
+        ok = many_wait1(&bar.qfull, np & 1, 1);
         if (!ok) break;
         ++np;
-        tc_fence_after();
-        if (ja == p.j0 && ja < jb) {
-          scores(0, nb & 1);
-          scores(1, nb & 1);
-        }
-        tc_commit(&bar.kempty[nb & 1]);
-        if (p.j1 == p.j0 + 1) tc_commit(&bar.qempty);
-#pragma unroll 1
-        for (int j = p.j0; j < p.j1; ++j) {
-          const uint32_t n = nb + j - p.j0, st = n & 1;
-          ok = many_wait1(&bar.vfull[st], (n >> 1) & 1, 1);
-          if (ok && many_edge(p, j)) {
-            ok = many_wait1(&bar.vfix[st], (fixes >> st) & 1, 1);
-            fixes ^= 1u << st;
-          }
-          if (ok && j + 1 < p.j1) ok = many_wait1(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, 1);
+        if (p.dual) {
+          // this half's blocks: every second one, in stages that are this half's alone (it gives
+          // both halves' word that they are free)
+          int j = p.j0 + ((nb + t) & 1);
+          uint32_t n = nb + j - p.j0;
+          for (int i = p.j0; i < p.j1; ++i)  // fix phases of the other half's blocks
+            if (many_edge(p, i) && ((i - j) & 1)) fixes ^= 1u << stage(nb + i - p.j0);
+          ok = many_wait1(&bar.kfull[stage(n)], phase(n), 1);
           if (!ok) break;
+          tc_fence_after();
+          scores(q_lo, 0, stage(n));
+          scores(q_lo, 1, stage(n));
+          tc_commit(&bar.kempty[stage(n)]);
+          tc_commit(&bar.kempty[stage(n)]);
+          if (j + 2 >= p.j1) tc_commit(&bar.qempty);
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            if (j >= ja && j < jb) {
+          for (; j < p.j1; j += 2, n += 2) {
+            ok = v_there(j, n);
+            if (!ok) break;
+            if (many_edge(p, j)) fixes ^= 1u << stage(n);
+            const bool again = j + 2 < p.j1;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
               ok = many_wait1(&bar.pfull[t][h], ns & 1, 3);
+              if (ok && again && h == 0) ok = many_wait1(&bar.kfull[stage(n + 2)], phase(n + 2), 1);
               if (!ok) break;
               tc_fence_after();
-              const uint32_t va = v_lo + st * (L::Tile >> 4) + h * (64 * 128 >> 4);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) tc_mma_ts(d_o, d_s + h * 64 + k * 8, va + k * (2048 >> 4), id_o);
-              tc_commit(&bar.odone[t][h]);
+              sums(h, stage(n));
+              if (again) scores(q_lo, h, stage(n + 2));
             }
-            if (j + 1 >= ja && j + 1 < jb) scores(h, (n + 1) & 1);
+            if (!ok) break;
+            ++ns;
+            if (again) {
+              tc_commit(&bar.kempty[stage(n + 2)]);
+              tc_commit(&bar.kempty[stage(n + 2)]);
+              if (j + 4 >= p.j1) tc_commit(&bar.qempty);
+            }
+            tc_commit(&bar.vempty[stage(n)]);
+            tc_commit(&bar.vempty[stage(n)]);
           }
           if (!ok) break;
-          ns += j >= ja && j < jb;
-          if (j + 1 < p.j1) {
-            tc_commit(&bar.kempty[(n + 1) & 1]);
-            if (j + 2 == p.j1) tc_commit(&bar.qempty);
+        } else {
+          ok = many_wait1(&bar.kfull[stage(nb)], phase(nb), 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (ja == p.j0 && ja < jb) {
+            scores(q_lo, 0, stage(nb));
+            scores(q_lo, 1, stage(nb));
           }
-          tc_commit(&bar.vempty[st]);
+          tc_commit(&bar.kempty[stage(nb)]);
+          if (p.j1 == p.j0 + 1) tc_commit(&bar.qempty);
+#pragma unroll 1
+          for (int j = p.j0; j < p.j1; ++j) {
+            const uint32_t n = nb + j - p.j0;
+            ok = v_there(j, n);
+            if (many_edge(p, j)) fixes ^= 1u << stage(n);
+            if (ok && j + 1 < p.j1) ok = many_wait1(&bar.kfull[stage(n + 1)], phase(n + 1), 1);
+            if (!ok) break;
+#pragma unroll 1
+            for (int h = 0; h < 2; ++h) {
+              if (j >= ja && j < jb) {
+                ok = many_wait1(&bar.pfull[t][h], ns & 1, 3);
+                if (!ok) break;
+                tc_fence_after();
+                sums(h, stage(n));
+              }
+              if (j + 1 >= ja && j + 1 < jb) scores(q_lo, h, stage(n + 1));
+            }
+            if (!ok) break;
+            ns += j >= ja && j < jb;
+            if (j + 1 < p.j1) {
+              tc_commit(&bar.kempty[stage(n + 1)]);
+              if (j + 2 == p.j1) tc_commit(&bar.qempty);
+            }
+            tc_commit(&bar.vempty[stage(n)]);
+          }
+          if (!ok) break;
         }
         nb += p.j1 - p.j0;
       }
-      // the last products' arrivals land before the block ends
-      if (ok && np > 0) {
-        many_wait1(&bar.kempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
-        many_wait1(&bar.qempty, (np - 1) & 1, 3);
-        many_wait1(&bar.vempty[(nb - 1) & 1], ((nb - 1) >> 1) & 1, 3);
-      }
+      // the last products and their arrivals end before the block does
+      tc_commit(&bar.drain[t]);
+      many_wait1(&bar.drain[t], 0, 3);
     }
     if (warp == 15 && lane == 0) {
       // ------------------------------------------------------------ parts
