@@ -1,22 +1,25 @@
 // The paged K/V cache: rows written (8 bits: quantised on the way) and read back.
 //
-// A row is the dim values of one (token, cache head).  DIM / 8 lanes hold it,
-// 8 values each: a warp takes 2 rows of 128 or 4 of 64, so its loads and stores
-// are whole 128-byte lines.  8 bits: the row's largest finite |x| comes from
-// shuffles over its lanes; its exponent e is the least one with
-// amax <= 448 * 2^e (448 = 1.75 * 2^8 is e4m3's largest value), so x * 2^-e is
-// exact in f32 and the only rounding is the one to e4m3.  A power of two costs
-// nothing against amax / 448 as a scale: e4m3's step is relative, only its
-// smallest values come a binade nearer to zero, and the attention can apply it
-// to exponents.  The places of a block's tokens (sequence by binary search of
-// cu_tokens, page from the table) are worked out once, in shared memory.
+// A row is the dim values of one (token, cache head).  DIM / 16 lanes hold it,
+// 16 values (32 bytes, 16 codes) each, two rows a thread at a time and six blocks
+// an SM: HBM bounds these kernels, so bytes in flight count (46k tokens x 16 heads x
+// 128 read back from 8 bits in 114 us, 5.0 TB/s; four rows a thread and four blocks
+// 120 us, 8 values a lane 158 us).  8 bits: the row's
+// largest finite |x| comes from shuffles over its lanes; its exponent e is the
+// least one with amax <= 448 * 2^e (448 = 1.75 * 2^8 is e4m3's largest value), so
+// x * 2^-e is exact in f32 and the only rounding is the one to e4m3.  A power of
+// two costs nothing against amax / 448 as a scale: e4m3's step is relative, only
+// its smallest values come a binade nearer to zero, and the attention can apply
+// it to exponents.  The places of a block's tokens are worked out once, in shared
+// memory: the block counts the sequences that begin before its first token (one
+// pass over cu_tokens, no chain of dependent loads), its tokens walk on from there.
 #include "cn_heads.cuh"
 
 namespace cn {
 namespace {
 
 constexpr int kKvThreads = 256;
-constexpr int kKvMaxTokens = 16;  // tokens of one block
+constexpr int kKvMaxTokens = 32;  // tokens of one block
 
 struct KvArgs {
   BatchArgs b;
@@ -27,25 +30,13 @@ struct KvArgs {
   int heads, per_block;
 };
 
-// Sequence of token row t, or -1: the last s with cu[s] <= t, t < cu[s + 1].
-__device__ __forceinline__ int seq_of(const BatchArgs& b, int t) {
-  int lo = 0, hi = b.n_seqs;  // cu[lo] <= t < cu[hi] if t belongs to a sequence
-  if (t < b.cu[0] || t >= b.cu[hi]) return -1;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (b.cu[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return lo;
-}
-
 // Cache row (of head 0) of token t: page * heads * page rows + row, or -1: no such
-// place (its row reads as zeros), or -2: t belongs to no sequence.
-__device__ __forceinline__ long long place_of(const KvArgs& a, long long t) {
-  const int s = seq_of(a.b, (int)t);
+// place (its row reads as zeros), or -2: t belongs to no sequence.  s: a sequence
+// that begins at t or before (or -1).
+__device__ __forceinline__ long long place_of(const KvArgs& a, long long t, int s) {
   if (s < 0) return -2;
+  while (s < a.b.n_seqs && a.b.cu[s + 1] <= t) ++s;
+  if (s >= a.b.n_seqs) return -2;
   const int pos = a.b.lengths[s] - a.b.cu[s + 1] + (int)t;
   if (pos < 0) return -1;
   const int page = page_of(a.b, s, pos);
@@ -61,15 +52,15 @@ __device__ __forceinline__ float group_max(float v) {
   return v;
 }
 
-// 8 values of a row to codes; every lane of the row gets the row's exponent byte.
+// 16 values of a row to codes; every lane of the row gets the row's exponent byte.
 template <typename T, int LANES>
-__device__ __forceinline__ uint2 quantise8(const uint4& raw, uint32_t* byte) {
-  float x[8];
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+__device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], uint32_t* byte) {
+  float x[16];
   float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = Num<T>::unpack(w[i]);
+  for (int i = 0; i < 8; ++i) {
+    const uint4& q = raw[i >> 2];
+    const float2 f = Num<T>::unpack((i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w);
     x[2 * i] = f.x;
     x[2 * i + 1] = f.y;
     amax = fmaxf(amax, fmaxf(isfinite(f.x) ? fabsf(f.x) : 0.f, isfinite(f.y) ? fabsf(f.y) : 0.f));
@@ -81,11 +72,11 @@ __device__ __forceinline__ uint2 quantise8(const uint4& raw, uint32_t* byte) {
   e = amax > 0.f ? min(max(e, -48), 48) : 0;
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
   *byte = (uint32_t)(e + 127);
-  uint32_t c[4];
+  uint32_t c[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)  // x - x is 0, or NaN where x is infinite: such a value becomes NaN, not 448
+  for (int i = 0; i < 8; ++i)  // x - x is 0, or NaN where x is infinite: such a value becomes NaN, not 448
     c[i] = floats_to_codes(fmaf(x[2 * i], inv, x[2 * i] - x[2 * i]), fmaf(x[2 * i + 1], inv, x[2 * i + 1] - x[2 * i + 1]));
-  return make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+  return make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
 }
 
 template <typename T>
@@ -116,22 +107,37 @@ __device__ __forceinline__ uint4 expand8(const uint2& codes, float scale) {
 
 // T: type of the rows.  CODED: 8-bit cache (else of type T too).  READ: cache -> rows.
 template <typename T, int DIM, bool CODED, bool READ>
-__global__ void __launch_bounds__(kKvThreads) k_kv(const KvArgs a) {
-  constexpr int LANES = DIM / 8;  // lanes of a row
+__global__ void __launch_bounds__(kKvThreads, 6) k_kv(const KvArgs a) {
+  constexpr int LANES = DIM / 16;  // lanes of a row
   constexpr int RPB = kKvThreads / LANES;  // rows that the block takes at a time
-  constexpr int U = 4;
+  constexpr int U = 2;
   __shared__ long long place[kKvMaxTokens];
+  __shared__ int began[kKvThreads / 32];
   pdl_trigger();
   pdl_wait();
   const long long t0 = (long long)blockIdx.x * a.per_block;
   const int nt = (int)min((long long)a.per_block, a.b.tokens - t0);
-  if (threadIdx.x < nt) place[threadIdx.x] = place_of(a, t0 + threadIdx.x);
+  int count = 0;  // sequences that begin at t0 or before (cu_tokens ascends)
+  for (int i = threadIdx.x; i < a.b.n_seqs; i += kKvThreads) count += a.b.cu[i] <= t0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xffffffffu, count, o);
+  if ((threadIdx.x & 31) == 0) began[threadIdx.x >> 5] = count;
+  __syncthreads();
+  if (threadIdx.x < nt) {
+    int s = -1;
+#pragma unroll
+    for (int w = 0; w < kKvThreads / 32; ++w) s += began[w];
+    const long long t = t0 + threadIdx.x;
+    // rows before the first sequence: one may begin behind t0
+    if (s < 0 && a.b.cu[0] <= t) s = 0;
+    place[threadIdx.x] = place_of(a, t, s);
+  }
   __syncthreads();
   const int lane = threadIdx.x % LANES;
   const int rows = nt * a.heads * 2;  // [token][k or v][head]
+  const uint32_t per_token = 2 * a.heads;
   for (int base = 0; base < rows; base += RPB * U) {
-    uint4 x[U];
-    uint2 c[U];
+    uint4 x[U][2], c[U];
     uint32_t byte[U];
     long long at[U];
     T* row[U];
@@ -141,24 +147,26 @@ __global__ void __launch_bounds__(kKvThreads) k_kv(const KvArgs a) {
       const int j = base + u * RPB + (int)threadIdx.x / LANES;
       at[u] = -2;
       byte[u] = 127;
-      x[u] = make_uint4(0, 0, 0, 0);
-      c[u] = make_uint2(0, 0);
+      x[u][0] = x[u][1] = c[u] = make_uint4(0, 0, 0, 0);
       if (j < rows) {
-        const int t = j / (2 * a.heads), r = j - t * 2 * a.heads;
-        v[u] = r >= a.heads;
+        const uint32_t t = (uint32_t)j / per_token, r = (uint32_t)j - t * per_token;
+        v[u] = r >= (uint32_t)a.heads;
         const int h = v[u] ? r - a.heads : r;
         at[u] = place[t];
         row[u] = static_cast<T*>(v[u] ? a.hv : a.hk) + (t0 + t) * (v[u] ? a.v_token : a.k_token) +
-                 h * (v[u] ? a.v_head : a.k_head) + lane * 8;
-        if (at[u] >= 0) at[u] += (long long)h << a.b.page_shift;
-        if constexpr (!READ) {
-          if (at[u] >= 0) x[u] = *reinterpret_cast<const uint4*>(row[u]);
-        } else if (at[u] >= 0) {
-          if constexpr (CODED) {
-            c[u] = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 8);
+                 h * (v[u] ? a.v_head : a.k_head) + lane * 16;
+        if (at[u] >= 0) {
+          at[u] += (long long)h << a.b.page_shift;
+          if constexpr (!READ) {
+            x[u][0] = reinterpret_cast<const uint4*>(row[u])[0];
+            x[u][1] = reinterpret_cast<const uint4*>(row[u])[1];
+          } else if constexpr (CODED) {
+            c[u] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 16);
             byte[u] = (v[u] ? a.ve : a.ke)[at[u]];
           } else {
-            x[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 8);
+            const uint4* p = reinterpret_cast<const uint4*>(static_cast<const T*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 16);
+            x[u][0] = p[0];
+            x[u][1] = p[1];
           }
         }
       }
@@ -166,16 +174,24 @@ __global__ void __launch_bounds__(kKvThreads) k_kv(const KvArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if constexpr (READ) {
-        if constexpr (CODED) x[u] = expand8<T>(c[u], exp_byte(byte[u]));
-        if (at[u] >= -1) *reinterpret_cast<uint4*>(row[u]) = x[u];
+        if constexpr (CODED) {
+          x[u][0] = expand8<T>(make_uint2(c[u].x, c[u].y), exp_byte(byte[u]));
+          x[u][1] = expand8<T>(make_uint2(c[u].z, c[u].w), exp_byte(byte[u]));
+        }
+        if (at[u] >= -1) {
+          reinterpret_cast<uint4*>(row[u])[0] = x[u][0];
+          reinterpret_cast<uint4*>(row[u])[1] = x[u][1];
+        }
       } else if constexpr (CODED) {
-        c[u] = quantise8<T, LANES>(x[u], &byte[u]);  // all lanes: it shuffles
+        c[u] = quantise16<T, LANES>(x[u], &byte[u]);  // all lanes: it shuffles
         if (at[u] >= 0) {
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 8) = c[u];
+          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 16) = c[u];
           if (lane == 0) (v[u] ? a.ve : a.ke)[at[u]] = (uint8_t)byte[u];
         }
       } else if (at[u] >= 0) {
-        *reinterpret_cast<uint4*>(static_cast<T*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 8) = x[u];
+        uint4* p = reinterpret_cast<uint4*>(static_cast<T*>(v[u] ? a.cv : a.ck) + at[u] * DIM + lane * 16);
+        p[0] = x[u][0];
+        p[1] = x[u][1];
       }
     }
   }
@@ -231,7 +247,8 @@ int kv_call(const char* who, bool read, const cn_kv_cache* cache, const cn_kv_ba
   a.v_token = v->token_stride;
   a.v_head = v->head_stride;
   a.heads = cache->heads;
-  a.per_block = tokens >= 16384 ? 16 : tokens >= 2048 ? 4 : 1;
+  // Enough blocks for all SMs several times over, each with enough rows to be worth its search.
+  a.per_block = (int)min((long long)kKvMaxTokens, max(1ll, tokens / (148 * 16)));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool coded = cache->dtype == CN_E4M3;
   cudaError_t e;
