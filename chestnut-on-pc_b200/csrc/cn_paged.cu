@@ -440,8 +440,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
     __syncthreads();
     const bool complete = u0 == 0 && u1 == units;
     const long long slot = 2ll * blockIdx.x + (u0 == 0 ? 1 : 0);
-    for (int x = tid; x < rows * (DIM / 4); x += kFewThreads) {
-      const int r = x / (DIM / 4), d = (x % (DIM / 4)) * 4;
+    // complete rows go out row by row, parts in the workspace's layout
+    for (int x = tid; x < kFewRows * (DIM / 4); x += kFewThreads) {
+      const int r = complete ? x / (DIM / 4) : x % kFewRows, d = (complete ? x % (DIM / 4) : x / kFewRows) * 4;
+      if (r >= rows) continue;
       float m = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, jm[(w * kFewRows + r) * 2]);
@@ -465,7 +467,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
                  (long long)(head * a.group + r - i * a.group) * a.o_head + d;
         *reinterpret_cast<uint2*>(out) = make_uint2(Num<T>::pack(sum.x * inv, sum.y * inv), Num<T>::pack(sum.z * inv, sum.w * inv));
       } else {
-        *reinterpret_cast<float4*>(a.part_o + (slot * kFewRows + r) * DIM + d) = sum;
+        *reinterpret_cast<float4*>(a.part_o + ((slot * (DIM / 4) + d / 4) * kFewRows + r) * 4) = sum;
         if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kFewRows + r) * 2) = make_float2(m, l);
       }
     }
@@ -477,52 +479,122 @@ __global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a)
   }
 }
 
-// Adds up the parts of a cut tile in their order.  grid (CTAs of the launch
-// before, row groups): block c looks at the boundary between CTAs c - 1 and c.
-// If it is the first one inside a tile, the tile's parts are the last one of
-// CTA c - 1 and the first ones of CTA c and of all behind it that begin inside.
-// A warp takes a row.
-template <typename T, int DIM, int ROWS, int RPB>
-__global__ void __launch_bounds__(RPB * 32) k_paged_merge(const PagedArgs a) {
-  pdl_trigger();
-  pdl_wait();
-  const int c = blockIdx.x + 1;
+// Adds up the parts of a cut tile in their order; one launch for both kernels.  A
+// block looks at the boundary between CTAs c - 1 and c of the launch before.  If
+// it is the first one inside a tile, the tile's parts are the last one of CTA
+// c - 1 and the first ones of CTA c and of all behind it that begin inside.
+// A block takes ROWS rows of it (all 16 of the few, 32 of the many), a thread 4 x
+// `Q` columns of a row, four parts at a time.  One context that is cut into
+// hundreds of parts is what takes long here: the few's parts are shared out
+// between four groups of threads, whose sums are joined in their order.
+template <typename T, int DIM, int TILE_ROWS, int ROWS, int GROUPS>
+__device__ __forceinline__ void paged_merge(const PagedArgs& a, int c, int row_group, float* smem) {
+  constexpr int COLS = 256 / ROWS / GROUPS;  // threads of a row (in a group)
+  constexpr int Q = DIM / 4 / COLS;          // float4s of a thread
+  constexpr int HALF = TILE_ROWS == 256 ? 128 : TILE_ROWS;
   const PagedCut cut = a.cuts[c];
   if (cut.start >= cut.total || cut.start <= cut.first || a.cuts[c - 1].start > cut.first) return;
   const PagedSeq sq = paged_seq(a, cut.seq);
-  const int r = blockIdx.y * RPB + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  // row r: of half r / HALF, there token i, query head h of the group
-  constexpr int HALF = ROWS == 256 ? 128 : ROWS;
+  const int r = row_group * ROWS + threadIdx.x % ROWS, col = threadIdx.x / ROWS % COLS, grp = threadIdx.x / ROWS / COLS;
+  // row r: of half r / HALF, there token i0, query head h of the group
   const int in_half = r % HALF, i0 = div_by(in_half, a.group, a.group_mul);
   const int i = r / HALF * a.half_tokens + i0, h = in_half - i0 * a.group;
-  if (i0 >= a.half_tokens || i >= paged_tokens(a, sq, cut.tile)) return;
+  const bool live = i0 < a.half_tokens && i < paged_tokens(a, sq, cut.tile);
   int last = c;  // the last CTA with a part
   while (last + 1 < a.ctas && a.cuts[last + 1].start < cut.first + cut.units) ++last;
-  constexpr int V = DIM / 32;
-  float m = -INFINITY, l = 0.f, o[V];
+  const int n = last - c + 2;
+  const int p0 = n * grp / GROUPS, p1 = n * (grp + 1) / GROUPS;
+  float m = -INFINITY, l = 0.f;
+  float4 o[Q];
 #pragma unroll
-  for (int x = 0; x < V; ++x) o[x] = 0.f;
-  for (int p = c - 1; p <= last; ++p) {
-    const long long slot = 2ll * p + (p == c - 1 ? 1 : 0);
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (slot * ROWS + r) * 2);
-    float f[V];
+  for (int x = 0; x < Q; ++x) o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live) {
+    constexpr int U = 4;
+    for (int p = p0; p < p1; p += U) {
+      float2 ml[U];
+      float4 f[U][Q];
 #pragma unroll
-    for (int x = 0; x < V; ++x) f[x] = a.part_o[(slot * ROWS + r) * DIM + x * 32 + lane];
-    const float n = fmaxf(m, ml.x);
-    const float co = m == -INFINITY ? 0.f : exp2_approx(m - n), cp = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - n);
-    m = n;
-    l = l * co + ml.y * cp;
+      for (int u = 0; u < U; ++u) {
+        ml[u] = make_float2(-INFINITY, 0.f);
+        if (p + u < p1) {
+          const long long slot = 2ll * (c - 1 + p + u) + (p + u == 0 ? 1 : 0);
+          ml[u] = *reinterpret_cast<const float2*>(a.part_ml + (slot * TILE_ROWS + r) * 2);
 #pragma unroll
-    for (int x = 0; x < V; ++x) o[x] = o[x] * co + f[x] * cp;
+          for (int x = 0; x < Q; ++x)
+            f[u][x] = *reinterpret_cast<const float4*>(a.part_o + ((slot * (DIM / 4) + col * Q + x) * TILE_ROWS + r) * 4);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (p + u >= p1) continue;
+        const float top = fmaxf(m, ml[u].x);
+        const float co = m == -INFINITY ? 0.f : exp2_approx(m - top), cp = ml[u].x == -INFINITY ? 0.f : exp2_approx(ml[u].x - top);
+        m = top;
+        l = l * co + ml[u].y * cp;
+#pragma unroll
+        for (int x = 0; x < Q; ++x) {
+          o[x].x = o[x].x * co + f[u][x].x * cp;
+          o[x].y = o[x].y * co + f[u][x].y * cp;
+          o[x].z = o[x].z * co + f[u][x].z * cp;
+          o[x].w = o[x].w * co + f[u][x].w * cp;
+        }
+      }
+    }
   }
+  if constexpr (GROUPS > 1) {
+    constexpr int PER = 256 / GROUPS;
+    float* mine = smem + threadIdx.x % PER;
+    float* ml = smem + (GROUPS - 1) * Q * 4 * PER + threadIdx.x % PER;
+    if (grp > 0) {
+#pragma unroll
+      for (int x = 0; x < Q; ++x) {
+        float* at = mine + (grp - 1) * Q * 4 * PER + x * 4 * PER;
+        at[0] = o[x].x, at[PER] = o[x].y, at[2 * PER] = o[x].z, at[3 * PER] = o[x].w;
+      }
+      ml[(grp - 1) * 2 * PER] = m;
+      ml[(grp - 1) * 2 * PER + PER] = l;
+    }
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) {
+      const float mg = ml[(g - 1) * 2 * PER], lg = ml[(g - 1) * 2 * PER + PER];
+      const float top = fmaxf(m, mg);
+      const float co = m == -INFINITY ? 0.f : exp2_approx(m - top), cp = mg == -INFINITY ? 0.f : exp2_approx(mg - top);
+      m = top;
+      l = l * co + lg * cp;
+#pragma unroll
+      for (int x = 0; x < Q; ++x) {
+        const float* at = mine + (g - 1) * Q * 4 * PER + x * 4 * PER;
+        o[x].x = o[x].x * co + at[0] * cp;
+        o[x].y = o[x].y * co + at[PER] * cp;
+        o[x].z = o[x].z * co + at[2 * PER] * cp;
+        o[x].w = o[x].w * co + at[3 * PER] * cp;
+      }
+    }
+  }
+  if (!live) return;
   const float inv = m == -INFINITY ? 0.f : 1.f / l;
   T* out = static_cast<T*>(a.out) + (long long)(sq.tok0 + cut.tile * a.tile_tokens + i) * a.o_token +
-           (long long)(cut.head * a.group + h) * a.o_head;
+           (long long)(cut.head * a.group + h) * a.o_head + col * Q * 4;
 #pragma unroll
-  for (int x = 0; x < V; ++x) {
-    const uint32_t w = Num<T>::pack(o[x] * inv, 0.f);
-    *reinterpret_cast<uint16_t*>(out + x * 32 + lane) = (uint16_t)w;
-  }
+  for (int x = 0; x < Q; ++x)
+    *reinterpret_cast<uint2*>(out + x * 4) = make_uint2(Num<T>::pack(o[x].x * inv, o[x].y * inv), Num<T>::pack(o[x].z * inv, o[x].w * inv));
+}
+
+constexpr int kManyMergeRows = 32;
+
+// grid: few_ctas - 1 blocks (none: 0), then 8 for each of many_ctas - 1 boundaries.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(256) k_paged_merge(const PagedArgs few, const PagedArgs many, int few_blocks) {
+  __shared__ float smem[3 * 64 * (DIM / 4 / 4 * 4 + 2)];
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x;
+  if (b < few_blocks)
+    paged_merge<T, DIM, kFewRows, kFewRows, 4>(few, b + 1, 0, smem);
+  else
+    paged_merge<T, DIM, 256, kManyMergeRows, 1>(many, (b - few_blocks) / 8 + 1, (b - few_blocks) % 8, smem);
 }
 
 }  // namespace

@@ -36,9 +36,10 @@ struct PagedArgs {
   int rows_min, rows_max;  // this launch takes the sequences with rows in [rows_min, rows_max]
   int ctas, min_units, snap, extra;
   struct PagedCut* cuts;   // [ctas + 1]
-  float* part_o;           // [2 * ctas][ROWS][DIM]
+  // A row's values in groups of four, rows beside each other: whole lines for a warp of rows.
+  float* part_o;           // [2 * ctas][DIM / 4][ROWS][4]
   float* part_ml;          // [2 * ctas][ROWS][2]
-  float* part_x;           // tcgen05 kernel: [ctas][2][2][128][DIM / 2], between the halves of a dual part
+  float* part_x;           // tcgen05 kernel: [ctas][2][2][DIM / 8][128][4], between the halves of a dual part
 };
 
 // Where CTA c's stretch begins: unit `start` of the line, inside tile (seq,

@@ -38,7 +38,7 @@ constexpr int kFewCtas = 2 * 148;  // two CTAs an SM
 constexpr int kManyCtas = 148;
 
 template <typename T, int DIM, bool CODED>
-cudaError_t few_launch(const PagedArgs& a, bool merge, int dev, cudaStream_t s) {
+cudaError_t few_launch(const PagedArgs& a, int dev, cudaStream_t s) {
   static unsigned long long ready = 0;
   if (dev >= 64 || !(ready & (1ull << dev))) {
     const cudaError_t e = cudaFuncSetAttribute(k_paged_few<T, DIM, CODED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -46,15 +46,11 @@ cudaError_t few_launch(const PagedArgs& a, bool merge, int dev, cudaStream_t s) 
     if (e != cudaSuccess) return e;
     if (dev < 64) ready |= 1ull << dev;
   }
-  cudaError_t e = launch_ex(k_paged_few<T, DIM, CODED>, dim3(a.ctas), dim3(kFewThreads), Few<DIM, CODED>::Smem, s, true, a);
-  if (e == cudaSuccess && merge)
-    e = launch_ex(k_paged_merge<T, DIM, kFewRows, 4>, dim3(a.ctas - 1, kFewRows / 4), dim3(128), 0, s, true, a);
-  return e;
+  return launch_ex(k_paged_few<T, DIM, CODED>, dim3(a.ctas), dim3(kFewThreads), Few<DIM, CODED>::Smem, s, true, a);
 }
 
 template <typename T, int DIM, bool CODED>
-cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, bool merge, int dev,
-                        cudaStream_t s) {
+cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int dev, cudaStream_t s) {
   static unsigned long long ready = 0;
   if (dev >= 64 || !(ready & (1ull << dev))) {
     cudaFuncAttributes at;
@@ -67,24 +63,24 @@ cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tk, const CUtenso
     if (e != cudaSuccess) return e;
     if (dev < 64) ready |= 1ull << dev;
   }
-  cudaError_t e = launch_ex(k_paged_many<T, DIM, CODED>, dim3(a.ctas), dim3(kManyThreads), Many<DIM>::Smem, s, true, tk, tv, a);
-  if (e == cudaSuccess && merge)
-    e = launch_ex(k_paged_merge<T, DIM, kManyRows, 8>, dim3(a.ctas - 1, kManyRows / 8), dim3(256), 0, s, true, a);
-  return e;
+  return launch_ex(k_paged_many<T, DIM, CODED>, dim3(a.ctas), dim3(kManyThreads), Many<DIM>::Smem, s, true, tk, tv, a);
 }
 
 // One call: the launches for few and for many rows (each where it may find work).
 struct PagedCall {
   PagedArgs few, many;
-  bool do_few, do_many, merge_few, merge_many;
+  bool do_few, do_many;
+  int merge_few, merge_many;  // blocks of the merge
   CUtensorMap tk, tv;
 };
 
 template <typename T, int DIM, bool CODED>
 cudaError_t paged_launch(const PagedCall& c, int dev, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
-  if (c.do_few) e = few_launch<T, DIM, CODED>(c.few, c.merge_few, dev, s);
-  if (e == cudaSuccess && c.do_many) e = many_launch<T, DIM, CODED>(c.many, c.tk, c.tv, c.merge_many, dev, s);
+  if (c.do_few) e = few_launch<T, DIM, CODED>(c.few, dev, s);
+  if (e == cudaSuccess && c.do_many) e = many_launch<T, DIM, CODED>(c.many, c.tk, c.tv, dev, s);
+  if (e == cudaSuccess && c.merge_few + c.merge_many)
+    e = launch_ex(k_paged_merge<T, DIM>, dim3(c.merge_few + c.merge_many), dim3(256), 0, s, true, c.few, c.many, c.merge_few);
   return e;
 }
 
@@ -199,9 +195,13 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
   a.window = window;
   // Sequences of up to 16 rows go to the kernel for few rows, the others to the
   // tensor-core one.  How long each is, only the device knows; a launch that
-  // cannot find work is left out, one that may not find any costs ~3 us.
+  // cannot find work is left out, and where no sequence can have more than 64 rows
+  // (each has a token or more) the first kernel takes them all, in tiles of 16
+  // rows: reading a context four times from L2 costs less than a launch that most
+  // likely finds nothing (~6 us).
   const long long rows = tokens * a.group;
-  const bool steps = tokens <= batch->n_seqs && a.group <= kFewRows;  // a token a sequence
+  const bool small = (tokens - batch->n_seqs + 1) * a.group <= 64 && tokens >= batch->n_seqs;
+  const bool steps = a.group <= kFewRows && (tokens <= batch->n_seqs || small);
   PagedCall c;
   memset(&c, 0, sizeof(c));
   c.do_few = batch->n_seqs > 1 ? a.group <= kFewRows : rows <= kFewRows;
@@ -219,7 +219,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     f.cuts = reinterpret_cast<PagedCut*>(w);
     f.part_o = reinterpret_cast<float*>(w + few.o);
     f.part_ml = reinterpret_cast<float*>(w + few.ml);
-    c.merge_few = cap > (long long)f.snap * kFewKeys;  // else no tile is ever cut
+    if (cap > (long long)f.snap * kFewKeys) c.merge_few = f.ctas - 1;  // else no tile is ever cut
   }
   if (c.do_many) {
     PagedArgs& m = c.many = a;
@@ -235,7 +235,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     m.part_o = reinterpret_cast<float*>(w + many.o);
     m.part_ml = reinterpret_cast<float*>(w + many.ml);
     m.part_x = reinterpret_cast<float*>(w + many.x);
-    c.merge_many = cap > (long long)m.snap * kManyKeys;
+    if (cap > (long long)m.snap * kManyKeys) c.merge_many = (m.ctas - 1) * (kManyRows / kManyMergeRows);
     if (!coded && (paged_map(&c.tk, cache, cache->k) || paged_map(&c.tv, cache, cache->v))) return CN_ERR_CUDA;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -598,25 +598,28 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       }
       int d0 = 0, d1 = DIM;  // the columns that this half writes out
       float c = 1.f, c2 = 0.f;
-      const float* theirs = nullptr;
+      const float4* theirs = nullptr;
       if (p.dual) {
         // Each half hands the other one its sums of the other one's columns (through L2: the
         // rings are full already of the next part) and joins its own.
-        float* mine = a.part_x + (((long long)blockIdx.x * 2 + (duals & 1)) * 2 + t) * 128 * (DIM / 2) + (long long)r * (DIM / 2);
+        float4* mine = reinterpret_cast<float4*>(a.part_x) +
+                       (((long long)blockIdx.x * 2 + (duals & 1)) * 2 + t) * (DIM / 8) * 128 + r;
 #pragma unroll 1
         for (int d = 0; d < DIM / 2; d += 32) {
           uint32_t o[32];
           tmem_ld32(to + (t ^ 1) * (DIM / 2) + d, o);
           tmem_ld_wait32(o);
-          st_row64(mine + d, o, true);
-          st_row64(mine + d + 16, o + 16, true);
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            mine[(d + i) / 4 * 128] = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
         }
         join_ml[duals & 1][t][r] = make_float2(m, l);
         mbar_arrive(&bar.joined);
         ok = many_wait(&bar.joined, duals & 1, 3);
         if (!ok) break;
         const float2 ml = join_ml[duals & 1][t ^ 1][r];
-        theirs = a.part_x + (((long long)blockIdx.x * 2 + (duals & 1)) * 2 + (t ^ 1)) * 128 * (DIM / 2) + (long long)r * (DIM / 2);
+        theirs = reinterpret_cast<const float4*>(a.part_x) +
+                 (((long long)blockIdx.x * 2 + (duals & 1)) * 2 + (t ^ 1)) * (DIM / 8) * 128 + r;
         ++duals;
         const float top = fmaxf(m, ml.x);
         c = m == -INFINITY ? 0.f : exp2_approx(m - top);
@@ -629,7 +632,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       const float inv = m == -INFINITY ? 0.f : 1.f / l;
       T* out = static_cast<T*>(a.out) + (long long)(p.seq_tok0 + p.tok0 + tok) * a.o_token +
                (long long)(p.head * a.group + my_h) * a.o_head;
-      const long long pr = slot * kManyRows + (p.dual ? 0 : t * 128) + r;
+      const int pr = (p.dual ? 0 : t * 128) + r;
       const bool wide = (reinterpret_cast<uintptr_t>(out) & 31) == 0;
 #pragma unroll 1
       for (int d = d0; d < d1; d += 32) {
@@ -644,7 +647,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if (p.dual) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(theirs + d - d0 + i));
+            const float4 x = __ldcg(theirs + (d - d0 + i) / 4 * 128);
             o[i] = __float_as_uint(fmaf(x.x, c2, __uint_as_float(o[i]) * c));
             o[i + 1] = __float_as_uint(fmaf(x.y, c2, __uint_as_float(o[i + 1]) * c));
             o[i + 2] = __float_as_uint(fmaf(x.z, c2, __uint_as_float(o[i + 2]) * c));
@@ -659,12 +662,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               w[i] = Num<T>::pack(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
             st_row64(out + d, w, wide);
           } else {
-            st_row64(a.part_o + pr * DIM + d, o, true);
-            st_row64(a.part_o + pr * DIM + d + 16, o + 16, true);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(a.part_o + ((slot * (DIM / 4) + (d + i) / 4) * kManyRows + pr) * 4) =
+                  make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
           }
         }
       }
-      if (live && !p.whole && d0 == 0) *reinterpret_cast<float2*>(a.part_ml + pr * 2) = make_float2(m, l);
+      if (live && !p.whole && d0 == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kManyRows + pr) * 2) = make_float2(m, l);
       tc_fence_before();  // the next part's zeros and products come after these loads
     }
   } else if (warp < 12) {
