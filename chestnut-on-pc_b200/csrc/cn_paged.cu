@@ -41,7 +41,7 @@ template <int DIM, bool CODED>
 struct Few {
   static constexpr int RB = DIM * (CODED ? 1 : 2);                    // bytes of a row
   static constexpr int Stage = 2 * kSlice * RB + (CODED ? 32 : 0);    // K, V and their 16 + 16 exponents
-  static constexpr int Stages = 24576 / (2 * kSlice * RB);            // 24 KB a warp: 3, 6 or 12 slices
+  static constexpr int Stages = (CODED ? 16384 : 24576) / (2 * kSlice * RB);  // a warp's ring: 3, 4, 6 or 8 slices
   static constexpr int Warp = Stage * Stages;
   static constexpr int Join = kFewWarps * kFewRows * (DIM + 4) * 4 + kFewWarps * kFewRows * 2 * 4;
   static constexpr size_t Smem = kFewWarps * Warp > Join ? kFewWarps * Warp : Join;
@@ -88,7 +88,7 @@ __device__ __forceinline__ int few_swizzle_v(int row, int ch) {
 
 // T: type of q, out (and of the cache unless CODED); M: of the products.
 template <typename T, int DIM, bool CODED>
-__global__ void __launch_bounds__(kFewThreads, 2) k_paged_few(const PagedArgs a) {
+__global__ void __launch_bounds__(kFewThreads, CODED ? 3 : 2) k_paged_few(const PagedArgs a) {
   using F = Few<DIM, CODED>;
   using M = std::conditional_t<CODED, __half, T>;
   constexpr int RB = F::RB, ST = F::Stages;

@@ -33,7 +33,7 @@ int sm_count(int dev) {
   return count[dev];
 }
 
-constexpr int kFewCtas = 2 * 148;  // two CTAs an SM
+constexpr int kFewCtas = 3 * 148;  // three CTAs an SM over an 8-bit cache, two over a 16-bit one
 
 constexpr int kManyCtas = 148;
 
@@ -195,12 +195,13 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
   a.window = window;
   // Sequences of up to 16 rows go to the kernel for few rows, the others to the
   // tensor-core one.  How long each is, only the device knows; a launch that
-  // cannot find work is left out, and where no sequence can have more than 64 rows
+  // cannot find work is left out, and where no sequence can have more than 128 rows
   // (each has a token or more) the first kernel takes them all, in tiles of 16
-  // rows: reading a context four times from L2 costs less than a launch that most
-  // likely finds nothing (~6 us).
+  // rows: one such sequence reads its context a few times from L2, which costs
+  // less than a launch that most likely finds nothing (48 sequences of 1 to 4
+  // tokens: 167 -> 151 us).
   const long long rows = tokens * a.group;
-  const bool small = (tokens - batch->n_seqs + 1) * a.group <= 64 && tokens >= batch->n_seqs;
+  const bool small = batch->n_seqs > 1 && (tokens - batch->n_seqs + 1) * a.group <= 128;
   const bool steps = a.group <= kFewRows && (tokens <= batch->n_seqs || small);
   PagedCall c;
   memset(&c, 0, sizeof(c));
@@ -212,7 +213,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     PagedArgs& f = c.few = a;
     f.rows_min = 1;
     f.rows_max = c.do_many ? kFewRows : INT32_MAX;
-    f.ctas = min(2 * sm_count(dev.device()), kFewCtas);
+    f.ctas = min((coded ? 3 : 2) * sm_count(dev.device()), kFewCtas);
     f.tile_tokens = f.half_tokens = kFewRows / a.group;
     f.min_units = f.snap = 4;
     f.extra = 1;

@@ -712,26 +712,25 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // 8-bit cache: a thread's codes of block j, 16 a piece; piece lt + 128 i
       constexpr int PR = DIM / 16;                 // pieces of a row
       constexpr int PT = CODED ? 128 * PR / 128 : 1;  // pieces of a thread
-      auto hold = [&](int j, const void* cache, uint4 (&c)[PT]) {
+      // (the pages of a block: lane l has that of keys 16 l .. 16 l + 15)
+      auto pages = [&](int j) {
+        const int key = p.lo + j * kManyKeys + lane * 16;
+        return j < p.j1 && lane < 8 && key < p.hi ? page_of(a.b, p.seq, key) : -1;
+      };
+      auto hold = [&](int j, int page, const void* cache, const uint8_t* exps, uint4 (&c)[PT]) -> uint32_t {
         const int k0 = p.lo + j * kManyKeys;
 #pragma unroll
         for (int i = 0; i < PT; ++i) {
-          const int key = k0 + (lt + 128 * i) / PR;
+          const int r = (lt + 128 * i) / PR, at = __shfl_sync(0xffffffffu, page, r >> 4);
           c[i] = make_uint4(0, 0, 0, 0);
-          if (key < p.hi) {
-            const int page = page_of(a.b, p.seq, key);
-            if (page >= 0) {
-              const long long kr = (((long long)page * a.heads + p.head) << shift) + (key & (page_rows - 1));
-              c[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + kr * DIM + ((lt + 128 * i) % PR) * 16);
-            }
+          if (at >= 0 && k0 + r < p.hi) {
+            const long long kr = (((long long)at * a.heads + p.head) << shift) + ((k0 + r) & (page_rows - 1));
+            c[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + kr * DIM + ((lt + 128 * i) % PR) * 16);
           }
         }
-      };
-      auto hold_exp = [&](int j, const uint8_t* exps) -> uint32_t {
-        const int key = p.lo + j * kManyKeys + lt;
-        if (key >= p.hi) return 127u;
-        const int page = page_of(a.b, p.seq, key);
-        return page < 0 ? 127u : exps[(((long long)page * a.heads + p.head) << shift) + (key & (page_rows - 1))];
+        const int at = __shfl_sync(0xffffffffu, page, lt >> 4);
+        if (at < 0 || k0 + lt >= p.hi) return 127u;
+        return exps[(((long long)at * a.heads + p.head) << shift) + ((k0 + lt) & (page_rows - 1))];
       };
       auto put = [&](const uint4 (&c)[PT], uint8_t* to) {
 #pragma unroll
@@ -755,10 +754,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       uint32_t ek = 0, ev = 0;
       int page = -1;
       if constexpr (CODED) {
-        hold(p.j0, a.k, ck);
-        ek = hold_exp(p.j0, a.k_exp);
-        hold(p.j0, a.v, cv);
-        ev = hold_exp(p.j0, a.v_exp);
+        page = pages(p.j0);
+        ek = hold(p.j0, page, a.k, a.k_exp, ck);
+        ev = hold(p.j0, page, a.v, a.v_exp, cv);
+        page = pages(p.j0 + 1);
       } else {
         if (warp == 8) {
           ok = fetch(p.j0, look_up(p.j0), nb, &tm_k, sk, bar.kfull, bar.kempty);
@@ -838,19 +837,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           kvx[st][lt >> 1][0][lt & 1] = exp_byte(ek) * a.scale;
           fence_proxy_async_smem();
           mbar_arrive(&bar.kfull[st]);
-          if (i + 1 < blocks) {
-            hold(j + 1, a.k, ck);
-            ek = hold_exp(j + 1, a.k_exp);
-          }
+          if (i + 1 < blocks) ek = hold(j + 1, page, a.k, a.k_exp, ck);
           put(cv, sv + st * L::Tile);
           kvx[st][lt >> 1][1][lt & 1] = (float)((int)ev - 127);
           vback[st][lt >> 1][lt & 1] = exp_byte(254u - ev);
           fence_proxy_async_smem();
           mbar_arrive(&bar.vfull[st]);
-          if (i + 1 < blocks) {
-            hold(j + 1, a.v, cv);
-            ev = hold_exp(j + 1, a.v_exp);
-          }
+          if (i + 1 < blocks) ev = hold(j + 1, page, a.v, a.v_exp, cv);
+          page = pages(j + 2);
         } else {
           if (warp == 8) {
             if (i + 1 < blocks) ok = fetch(j + 1, page, n + 1, &tm_k, sk, bar.kfull, bar.kempty);
