@@ -192,7 +192,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
   a.group_mul = a.group == 1 ? 0xffffffffu : (uint32_t)((1ull << 32) / (uint32_t)a.group);
   a.scale = scale * 1.44269504088896340736f;
   a.causal = causal != 0;
-  a.window = window;
+  a.window = min(window, 1 << 30);  // positions end below it
   // Sequences of up to 16 rows go to the kernel for few rows, the others to the
   // tensor-core one.  How long each is, only the device knows; a launch that
   // cannot find work is left out, and where no sequence can have more than 128 rows

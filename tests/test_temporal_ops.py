@@ -162,12 +162,13 @@ def test_kv_read_refuses_overlapping_outputs():
     dict(q=_heads(h=12)), dict(q=_heads(h=4)), dict(q=_heads(d=128), out=_heads(d=128)), dict(out=_heads(h=16)),
     dict(q=_heads(dtype="bf16"), out=_heads(dtype="bf16")), dict(q=_heads(dtype="f32"), out=_heads(dtype="f32")),
     dict(out=_heads(dtype="bf16")), dict(window=-1), dict(window=4, causal=0), dict(out=_heads(ts=64)),
+    dict(q=_heads(h=1032), out=_heads(h=1032)), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan),
     dict(work=None), dict(work=0xa0010), dict(bytes=1000), dict(tokens=-1), dict(tokens=(1 << 30) + 1),
 ])
 def test_attention_refuses(args):
     a = dict(cache=_cache(), batch=_batch(), q=_heads(), out=_heads(ptr=0x90000), tokens=16, causal=1, window=0,
-             work=0xa0000, bytes=1 << 40) | args
-    rc = _lib.lib().cn_paged_attention(a["cache"], a["batch"], a["q"], a["out"], a["tokens"], 0.125, a["causal"],
+             work=0xa0000, bytes=1 << 40, scale=0.125) | args
+    rc = _lib.lib().cn_paged_attention(a["cache"], a["batch"], a["q"], a["out"], a["tokens"], a["scale"], a["causal"],
                                        a["window"], a["work"], a["bytes"], None)
     assert rc == CN_ERR_ARG and _lib.lib().cn_last_error().startswith(b"cn_paged_attention")
 
@@ -397,6 +398,84 @@ def test_attention_against_64_bits(shape):
     assert kernels.device_error() == 0
     again = attend(st, causal=causal, window=window)
     assert torch.equal(out, again)
+
+
+LARGE = [
+    # dtype, cache, dim, page, cache heads, group, new, past, causal, window
+    ("bf16", "bf16", 128, 64, 2, 3, [700, 64, 1, 0, 17], [0, 3000, 5000, 10, 900], True, 0),  # both kernels, one merge
+    ("f16", "f16", 128, 16, 1, 1, [64], [20000], False, 0),        # one tile of one half over every CTA
+    ("f16", "f16", 128, 256, 1, 1, [1], [30000], True, 0),         # one row in hundreds of parts
+    ("f16", "e4m3", 64, 32, 1, 2, [1, 2], [40000, 3], True, 0),
+    ("f16", "e4m3", 64, 128, 2, 3, [1500, 300], [0, 2000], True, 333),
+    ("bf16", "e4m3", 128, 64, 1, 4, [513], [1111], True, 0),
+    ("bf16", "bf16", 64, 64, 1, 128, [1, 3], [700, 40], True, 0),  # the largest group
+    ("f16", "f16", 64, 16, 1, 40, [1, 1, 9], [5000, 0, 77], True, 0),
+    ("f16", "e4m3", 128, 16, 2, 20, [2, 1], [300, 4000], True, 1000),
+    ("f16", "f16", 128, 128, 4, 1, [2048], [0], True, 0),
+    ("bf16", "bf16", 64, 32, 3, 5, [255, 256, 257], [129, 127, 128], True, 128),
+    ("f16", "f16", 128, 64, 1, 1, [129, 128, 127, 1], [640, 64, 0, 0], False, 0),
+    ("f16", "f16", 64, 16, 2, 2, [1] * 300 + [40], list(range(300)) + [1000], True, 0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("shape", LARGE, ids=lambda s: "-".join(map(str, s[:6])) + f"-{len(s[6])}seqs-{max(s[6])}-{max(s[7])}")
+def test_attention_over_long_contexts(shape):
+    """Cut tiles, merges, halves that share a tile's keys: against 64 bits on the GPU, sequence by sequence."""
+    dtype, cache, dim, page, hk, group, new, past, causal, window = shape
+    g = torch.Generator(device="cuda").manual_seed(7)
+    n, hq = len(new), hk * group
+    length = [a + b for a, b in zip(new, past)]
+    used = [-(-v // page) for v in length]
+    pages, width = sum(used) + 2, max(used)
+    order = torch.randperm(pages, generator=g, device="cuda").int()
+    table = torch.full((n, width), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for s in range(n):
+        table[s, : used[s]] = order[at:at + used[s]]
+        at += used[s]
+    body, exps, wide = {}, {}, {}
+    for m in "kv":
+        x = torch.randn(pages, hk, page, dim, generator=g, device="cuda") * (0.3 + 3 * torch.rand(pages, hk, page, 1, generator=g, device="cuda") ** 3)
+        if cache == "e4m3":
+            part, e = torch.frexp(x.abs().amax(-1))
+            e = e - 9 + (part > 0.875).int()
+            power = lambda k: ((k + 127) << 23).view(torch.float32)[..., None]  # noqa: E731
+            codes = (x * power(-e)).to(torch.float8_e4m3fn)
+            wide[m] = codes.double() * power(e).double()
+            body[m], exps[m] = codes.view(torch.uint8), (e + 127).to(torch.uint8)
+        else:
+            body[m], exps[m] = x.to(TYPES[dtype]), None
+            wide[m] = body[m].double()
+    q = torch.randn(sum(new) + 1, hq, dim, generator=g, device="cuda").to(TYPES[dtype])
+    st = dict(dtype=dtype, cache=cache, dim=dim, page=page, hk=hk, group=group, new=new, past=past, pages=pages, width=width,
+              k=body["k"], v=body["v"], k_exp=exps["k"], v_exp=exps["v"], d_table=table, d_qkv=q,
+              d_cu=torch.tensor([0] + np.cumsum(new).tolist(), dtype=torch.int32).cuda(), d_len=torch.tensor(length, dtype=torch.int32).cuda())
+    out = attend(st, causal=causal, window=window)
+    assert kernels.device_error() == 0
+    assert torch.equal(out, attend(st, causal=causal, window=window))
+    row = 0
+    for s in range(n):
+        keys = torch.arange(length[s], device="cuda")
+        k, v = (wide[m][table[s].long()[keys // page], :, keys % page] for m in "kv")  # [keys, hk, dim]
+        pos = past[s] + torch.arange(new[s], device="cuda")[:, None]
+        for h in range(hq):
+            kk, vv = k[:, h // group], v[:, h // group]
+            qq = q[row:row + new[s], h].double()
+            a = qq @ kk.T * dim ** -0.5
+            if causal:
+                a[keys > pos] = -math.inf
+            if window:
+                a[keys <= pos - window] = -math.inf
+            w = torch.softmax(a, -1)
+            big = (qq.abs() @ kk.abs().T * dim ** -0.5).amax(-1, keepdim=True)
+            err = 2 * (dim + 4) * U32 * big + 2.0 ** -21 + length[s] * U32
+            tol = tiny(dtype) + u(dtype) * (w @ vv).abs() + (u("f16" if cache == "e4m3" else dtype) + err) * (w @ vv.abs()) \
+                + 2 * length[s] * 2.0 ** -25 * (w * vv.abs().amax(-1)).amax(-1, keepdim=True)
+            off = (out[row:row + new[s], h].double() - w @ vv).abs() - tol * (1 + u(dtype))
+            assert new[s] == 0 or off.max() <= 0, (s, h, off.max())
+        row += new[s]
+    assert torch.all(out[row:] == 7.0)
 
 
 @gpu
