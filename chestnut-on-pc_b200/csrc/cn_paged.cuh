@@ -31,6 +31,7 @@ struct PagedArgs {
   int heads, group;     // cache heads, query heads of each
   uint32_t group_mul;   // divides rows by group: see div_by
   int tile_tokens, half_tokens;
+  int q_map;            // tcgen05 kernel: Q comes by TMA
   float scale;          // the caller's scale * log2(e)
   int causal, window;
   int rows_min, rows_max;  // this launch takes the sequences with rows in [rows_min, rows_max]

@@ -50,7 +50,8 @@ cudaError_t few_launch(const PagedArgs& a, int dev, cudaStream_t s) {
 }
 
 template <typename T, int DIM, bool CODED>
-cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tk, const CUtensorMap& tv, int dev, cudaStream_t s) {
+cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, int dev,
+                        cudaStream_t s) {
   static unsigned long long ready = 0;
   if (dev >= 64 || !(ready & (1ull << dev))) {
     cudaFuncAttributes at;
@@ -63,7 +64,7 @@ cudaError_t many_launch(const PagedArgs& a, const CUtensorMap& tk, const CUtenso
     if (e != cudaSuccess) return e;
     if (dev < 64) ready |= 1ull << dev;
   }
-  return launch_ex(k_paged_many<T, DIM, CODED>, dim3(a.ctas), dim3(kManyThreads), Many<DIM>::Smem, s, true, tk, tv, a);
+  return launch_ex(k_paged_many<T, DIM, CODED>, dim3(a.ctas), dim3(kManyThreads), Many<DIM>::Smem, s, true, tq, tk, tv, a);
 }
 
 // One call: the launches for few and for many rows (each where it may find work).
@@ -71,14 +72,14 @@ struct PagedCall {
   PagedArgs few, many;
   bool do_few, do_many;
   int merge_few, merge_many;  // blocks of the merge
-  CUtensorMap tk, tv;
+  CUtensorMap tq, tk, tv;
 };
 
 template <typename T, int DIM, bool CODED>
 cudaError_t paged_launch(const PagedCall& c, int dev, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (c.do_few) e = few_launch<T, DIM, CODED>(c.few, dev, s);
-  if (e == cudaSuccess && c.do_many) e = many_launch<T, DIM, CODED>(c.many, c.tk, c.tv, dev, s);
+  if (e == cudaSuccess && c.do_many) e = many_launch<T, DIM, CODED>(c.many, c.tq, c.tk, c.tv, dev, s);
   if (e == cudaSuccess && c.merge_few + c.merge_many)
     e = launch_ex(k_paged_merge<T, DIM>, dim3(c.merge_few + c.merge_many), dim3(256), 0, s, true, c.few, c.many, c.merge_few);
   return e;
@@ -97,6 +98,19 @@ int paged_map(CUtensorMap* m, const cn_kv_cache* c, const void* base) {
   const uint32_t b[3] = {64, (uint32_t)(c->page < kManyKeys ? c->page : kManyKeys), 1};
   return encode(m, c->dtype == CN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, d,
                 st, b, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// The queries as [tokens][heads][dim], boxes of one half of a tile.  Strides of 0 (rows that are
+// the same memory) are left to the kernel's own loads.
+bool paged_q_map(CUtensorMap* m, const cn_heads* q, long long tokens, int group, int half_tokens) {
+  if ((q->heads > 1 && q->head_stride == 0) || (tokens > 1 && q->token_stride == 0)) return false;
+  const uint64_t row = (uint64_t)q->dim * 2;
+  const uint64_t d[3] = {(uint64_t)q->dim, (uint64_t)q->heads, (uint64_t)tokens};
+  const uint64_t st[2] = {q->heads > 1 ? (uint64_t)q->head_stride * 2 : row, tokens > 1 ? (uint64_t)q->token_stride * 2 : row};
+  if (st[0] >= 1ull << 40 || st[1] >= 1ull << 40) return false;
+  const uint32_t b[3] = {64, (uint32_t)group, (uint32_t)half_tokens};
+  return encode(m, q->dtype == CN_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, q->data, d, st,
+                b, CU_TENSOR_MAP_SWIZZLE_128B) == 0;
 }
 
 int paged_check(const char* who, const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
@@ -237,6 +251,8 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
     m.part_ml = reinterpret_cast<float*>(w + many.ml);
     m.part_x = reinterpret_cast<float*>(w + many.x);
     if (cap > (long long)m.snap * kManyKeys) c.merge_many = (m.ctas - 1) * (kManyRows / kManyMergeRows);
+    // (bf16 rows over an 8-bit cache are scaled to f16 on their way)
+    m.q_map = !(coded && q->dtype == CN_BF16) && paged_q_map(&c.tq, q, tokens, m.group, m.half_tokens);
     if (!coded && (paged_map(&c.tk, cache, cache->k) || paged_map(&c.tv, cache, cache->v))) return CN_ERR_CUDA;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);

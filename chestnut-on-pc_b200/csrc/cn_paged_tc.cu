@@ -294,7 +294,8 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
 // T: q and out (and a 16-bit cache).
 template <typename T, int DIM, bool CODED>
 __global__ void __launch_bounds__(kManyThreads, 1)
-    k_paged_many(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
+    k_paged_many(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ CUtensorMap tm_v, const PagedArgs a) {
   using L = Many<DIM>;
   using M = std::conditional_t<CODED, __half, T>;
   using R = ManyRegs<CODED>;
@@ -337,6 +338,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     mbar_init(&bar.qempty, 2);
     mbar_init(&bar.asked, 1);
     fence_barrier_init();
+    if (a.q_map) tma_prefetch_desc(&tm_q);
     if constexpr (!CODED) {
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
@@ -826,13 +828,24 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             if (i % CH == 0) qpow[(np - 1) & 1][i / CH] = __uint_as_float((eb - 13u) << 23);
           }
         }
+      } else if (a.q_map) {
+        // a box is a half: half_tokens tokens x the group's heads x 64 values.  What of it belongs to
+        // no token of this part are other rows, whose results nobody reads.
+        if (lt == 0) {
+          mbar_arrive_expect_tx(&bar.qfull, (uint32_t)(qrows / 128 * a.half_tokens * a.group * DIM * 2));
+          for (int t = 0; t < qrows / 128; ++t)
+#pragma unroll
+            for (int d = 0; d < DIM / 64; ++d)
+              tma_load_3d(sq + t * L::Tile + d * L::Sub, &tm_q, &bar.qfull, d * 64, p.head * a.group,
+                          p.seq_tok0 + p.tok0 + t * a.half_tokens);
+        }
       } else {
 #pragma unroll 4
         for (int i = lt; i < qrows * CH; i += 128) cp_async16(q_dst(i), q_src(i));
         cp_async_wait_all();
       }
       fence_proxy_async_smem();
-      mbar_arrive(&bar.qfull);
+      if (lt != 0 || !a.q_map) mbar_arrive(&bar.qfull);
 
       // ---- blocks
       for (int i = 0; i < blocks && ok; ++i) {
