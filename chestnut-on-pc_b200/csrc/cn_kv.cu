@@ -2,10 +2,13 @@
 //
 // A row is the dim values of one (token, cache head).  DIM / 16 lanes hold it,
 // 16 values (32 bytes, 16 codes) each, two rows a thread at a time and six blocks
-// an SM: HBM bounds these kernels, so bytes in flight count (46k tokens x 16 heads x
-// 128 read back from 8 bits in 114 us, 5.0 TB/s; four rows a thread and four blocks
-// 120 us, 8 values a lane 158 us).  8 bits: the row's
-// largest finite |x| comes from shuffles over its lanes; its exponent e is the
+// an SM.  HBM bounds these kernels, so bytes in flight count, and few instructions
+// a value: 46k tokens x 16 heads x 128 are read back from 8 bits to bf16 in 106 us
+// (5.4 TB/s, 82% of the copy rate; with every value's range checked 117 us, with
+// four rows a thread and four blocks 120 us, with 8 values a lane 158 us), 18k
+// tokens x 8 heads x 128 bf16 are written in 25 us (4.5 TB/s, 68%; 27 us with the
+// finite test on every value).  8 bits: the row's largest finite |x| comes from
+// maxima of pairs and shuffles over its lanes; its exponent e is the
 // least one with amax <= 448 * 2^e (448 = 1.75 * 2^8 is e4m3's largest value), so
 // x * 2^-e is exact in f32 and the only rounding is the one to e4m3.  A power of
 // two costs nothing against amax / 448 as a scale: e4m3's step is relative, only
@@ -13,6 +16,8 @@
 // it to exponents.  The places of a block's tokens are worked out once, in shared
 // memory: the block counts the sequences that begin before its first token (one
 // pass over cu_tokens, no chain of dependent loads), its tokens walk on from there.
+#include <type_traits>
+
 #include "cn_heads.cuh"
 
 namespace cn {
@@ -52,20 +57,42 @@ __device__ __forceinline__ float group_max(float v) {
   return v;
 }
 
+// Larger of pairs of 16-bit values (a NaN loses against a number).
+template <typename T>
+__device__ __forceinline__ uint32_t max_pairs(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t max_pairs<__half>(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <>
+__device__ __forceinline__ uint32_t max_pairs<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
 // 16 values of a row to codes; every lane of the row gets the row's exponent byte.
 template <typename T, int LANES>
 __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], uint32_t* byte) {
-  float x[16];
-  float amax = 0.f;
+  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+  uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint4& q = raw[i >> 2];
-    const float2 f = Num<T>::unpack((i & 3) == 0 ? q.x : (i & 3) == 1 ? q.y : (i & 3) == 2 ? q.z : q.w);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
-    amax = fmaxf(amax, fmaxf(isfinite(f.x) ? fabsf(f.x) : 0.f, isfinite(f.y) ? fabsf(f.y) : 0.f));
+  for (int i = 0; i < 8; ++i) top = max_pairs<T>(top, w[i] & 0x7fff7fffu);
+  const float2 two = Num<T>::unpack(top);
+  float amax = group_max<LANES>(fmaxf(two.x, two.y));
+  // (the warp decides together: group_max below is for all lanes)
+  const bool infinite = __any_sync(0xffffffffu, isinf(amax));
+  if (infinite) {  // the largest finite one then
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 f = Num<T>::unpack(w[i]);
+      amax = fmaxf(amax, fmaxf(isfinite(f.x) ? fabsf(f.x) : 0.f, isfinite(f.y) ? fabsf(f.y) : 0.f));
+    }
+    amax = group_max<LANES>(amax);
   }
-  amax = group_max<LANES>(amax);
   // amax = 1.m * 2^k; 448 * 2^e >= amax  <=>  e >= k - 8, or k - 7 where 1.m > 1.75
   const uint32_t bits = __float_as_uint(amax);
   int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
@@ -74,32 +101,43 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], uint32_t* byt
   *byte = (uint32_t)(e + 127);
   uint32_t c[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)  // x - x is 0, or NaN where x is infinite: such a value becomes NaN, not 448
-    c[i] = floats_to_codes(fmaf(x[2 * i], inv, x[2 * i] - x[2 * i]), fmaf(x[2 * i + 1], inv, x[2 * i + 1] - x[2 * i + 1]));
+  for (int i = 0; i < 8; ++i) {
+    float2 f = Num<T>::unpack(w[i]);
+    if (infinite) {  // x - x is NaN where x is infinite: such a value becomes NaN, not 448
+      f.x += f.x - f.x;
+      f.y += f.y - f.y;
+    }
+    c[i] = floats_to_codes(f.x * inv, f.y * inv);
+  }
   return make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
 }
 
+// 8 codes to 8 values of T, times 2^(byte - 127).
 template <typename T>
-__device__ __forceinline__ float finite_limit();
-template <>
-__device__ __forceinline__ float finite_limit<__half>() { return 65504.f; }
-template <>
-__device__ __forceinline__ float finite_limit<__nv_bfloat16>() { return __uint_as_float(0x7f7f0000u); }
-
-// 8 codes to 8 values of T.
-template <typename T>
-__device__ __forceinline__ uint4 expand8(const uint2& codes, float scale) {
+__device__ __forceinline__ uint4 expand8(const uint2& codes, uint32_t byte) {
   const uint32_t c[4] = {codes.x & 0xffffu, codes.x >> 16, codes.y & 0xffffu, codes.y >> 16};
   uint32_t w[4];
-  constexpr float kMax = 3.4e38f;
+  if constexpr (std::is_same_v<T, __half>) {
+    // 2^-24 .. 2^7: the power is an f16 number and no product is beyond f16 (448 * 2^7 < 65504); it is
+    // rounded once, as from f32
+    if (byte >= 103u && byte <= 134u) {
+      const uint32_t p = byte >= 113u ? (byte - 112u) << 10 : 1u << (byte - 103u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(w[i]) : "r"(codes_to_h2(c[i])), "r"(p | p << 16));
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  const float scale = exp_byte(byte);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = Num<__half>::unpack(codes_to_h2(c[i]));
     float a = f.x * scale, b = f.y * scale;
-    // finite values beyond T's range become its largest (NaN passes: both comparisons fail)
-    const float lim = finite_limit<T>();
-    a = fabsf(a) > lim && fabsf(a) < kMax ? copysignf(lim, a) : a;
-    b = fabsf(b) > lim && fabsf(b) < kMax ? copysignf(lim, b) : b;
+    if constexpr (std::is_same_v<T, __half>) {
+      // finite values beyond f16 become its largest (fminf and fmaxf would make one of a NaN; bf16 holds all that
+      // cn_kv_write's exponents can make)
+      a = fabsf(a) > 65504.f ? copysignf(65504.f, a) : a;
+      b = fabsf(b) > 65504.f ? copysignf(65504.f, b) : b;
+    }
     w[i] = Num<T>::pack(a, b);
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
@@ -175,8 +213,8 @@ __global__ void __launch_bounds__(kKvThreads, 6) k_kv(const KvArgs a) {
     for (int u = 0; u < U; ++u) {
       if constexpr (READ) {
         if constexpr (CODED) {
-          x[u][0] = expand8<T>(make_uint2(c[u].x, c[u].y), exp_byte(byte[u]));
-          x[u][1] = expand8<T>(make_uint2(c[u].z, c[u].w), exp_byte(byte[u]));
+          x[u][0] = expand8<T>(make_uint2(c[u].x, c[u].y), byte[u]);
+          x[u][1] = expand8<T>(make_uint2(c[u].z, c[u].w), byte[u]);
         }
         if (at[u] >= -1) {
           reinterpret_cast<uint4*>(row[u])[0] = x[u][0];
