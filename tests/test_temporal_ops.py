@@ -821,6 +821,99 @@ def test_a_run_of_steps(dtype, cache, dim, page):
 
 
 @gpu
+@pytest.mark.parametrize("cache,dtype", [("f16", "f16"), ("e4m3", "bf16")])
+def test_rows_before_the_first_sequence_and_repeated_queries(cache, dtype):
+    """cu_tokens that begin behind row 0; queries whose tokens are one row in memory (token stride 0)."""
+    st = make(dtype, cache, 64, 16, 2, 2, [40, 1], [30, 100], tail_rows=0)
+    ref = attend(st)
+    check_attention(st, ref)
+    st["d_cu"] += 3
+    shifted = torch.cat([st["d_qkv"][:3], st["d_qkv"], st["d_qkv"][:2]])
+    moved = dict(st, d_qkv=shifted)
+    out = attend(moved)
+    assert torch.equal(out[3:-2], ref) and torch.all(out[:3] == 7.0) and torch.all(out[-2:] == 7.0)
+    st["d_cu"] -= 3
+    one = torch.randn(1, 4, 64, device="cuda").to(TYPES[dtype])
+    same = dict(st, d_qkv=one.expand(41, 4, 64), qkv=one.expand(41, 4, 64).cpu())
+    check_attention(same, attend(same))
+    k = torch.full((46, 2, 64), 2.0, device="cuda", dtype=TYPES[dtype])
+    st["d_cu"] += 3
+    c, b = descriptors(st)
+    back = torch.full_like(k, 9.0)
+    kernels.kv_write(c, b, handle(k, dtype), handle(k, dtype), 46, stream())
+    kernels.kv_read(c, b, handle(back, dtype), handle(back.clone(), dtype), 46, stream())
+    assert torch.all(back[3:44] == 2.0) and torch.all(back[:3] == 9.0) and torch.all(back[44:] == 9.0)
+    assert kernels.device_error() == 0
+
+
+@gpu
+def test_sequences_without_a_table():
+    """Contexts of length 0 need no pages: zeros; a length without pages is reported."""
+    q = torch.randn(3, 2, 64, device="cuda").half()
+    cu, lens = torch.tensor([0, 2, 3], dtype=torch.int32).cuda(), torch.tensor([0, 0], dtype=torch.int32).cuda()
+    k = torch.zeros(1, 2, 16, 64, device="cuda", dtype=torch.float16)
+    cache = kernels.kv_cache(k.data_ptr(), k.data_ptr(), "f16", 1, 16, 2, 64)
+    batch = kernels.kv_batch(2, cu.data_ptr(), lens.data_ptr(), None, 0)
+    nb = kernels.paged_attention_workspace(cache, batch, handle(q, "f16"), 3)
+    work, out = torch.empty(nb, device="cuda", dtype=torch.uint8), torch.ones_like(q)
+    for length, code in ((0, 0), (5, 6)):
+        lens.fill_(length)
+        kernels.paged_attention(cache, batch, handle(q, "f16"), handle(out.fill_(1), "f16"), 3, 0.125, True, 0, work.data_ptr(), nb, stream())
+        torch.cuda.synchronize()
+        assert torch.all(out == 0) and kernels.device_error() == code
+
+
+@gpu
+def test_two_calls_at_once():
+    """Two streams, each with a workspace of its own, over one cache."""
+    st = make("f16", "f16", 128, 64, 2, 2, [90, 1, 5], [300, 2000, 0], tail_rows=0)
+    ref = attend(st)
+    check_attention(st, ref)
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i in (0, 1):
+            with torch.cuda.stream(side[i]):
+                outs[i].append(attend(st))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref) for o in outs[0] + outs[1])
+
+
+@gpu
+def test_calls_without_torch():
+    """A step on the package's own buffers, as a host without PyTorch makes it: packed q|k|v, 8-bit cache."""
+    from chestnut_b200 import DeviceBuffer
+    rs = np.random.default_rng(0)
+    tokens, page, pages, width = 3, 64, 6, 3
+    qkv = rs.standard_normal((tokens, 48, 128)).astype(np.float16)
+    d_qkv = DeviceBuffer(qkv.nbytes).upload(qkv)
+    k, v = (DeviceBuffer(pages * 16 * page * 128).zero() for _ in range(2))
+    ke, ve = (DeviceBuffer(pages * 16 * page).zero() for _ in range(2))
+    i32 = [DeviceBuffer(a.nbytes).upload(a) for a in (np.array([0, 1, 2, 3], np.int32), np.array([1, 1, 1], np.int32),
+                                                      np.arange(9, dtype=np.int32).reshape(3, 3) % 6)]
+    cache = kernels.kv_cache(k.ptr, v.ptr, "e4m3", pages, page, 16, 128, ke.ptr, ve.ptr)
+    table = np.array([[0, 1, 2], [3, 4, 5], [5, 1, 1]], np.int32)
+    i32[2].upload(table)
+    batch = kernels.kv_batch(tokens, *(b.ptr for b in i32), width)
+    q, kk, vv = (kernels.heads(d_qkv.ptr + i * 16 * 128 * 2, "f16", 16, 128, 48 * 128) for i in range(3))
+    qk = kernels.heads(d_qkv.ptr, "f16", 32, 128, 48 * 128)
+    freq, magnitude = kernels.rope_frequencies(128, factor=8.0, scaling="parts", context=4096)
+    pos, d_freq = np.zeros(tokens, np.int64), DeviceBuffer(freq.nbytes).upload(freq)
+    d_pos, d_out = DeviceBuffer(pos.nbytes).upload(pos), DeviceBuffer(tokens * 16 * 128 * 2)
+    out = kernels.heads(d_out.ptr, "f16", 16, 128)
+    work = DeviceBuffer(kernels.paged_attention_workspace(cache, batch, q, tokens))
+    kernels.rope(qk, qk, tokens, d_pos.ptr, d_freq.ptr, 128, magnitude=magnitude)
+    kernels.kv_write(cache, batch, kk, vv, tokens)
+    kernels.paged_attention(cache, batch, q, out, tokens, 128 ** -0.5, True, 0, work.ptr, work.nbytes)
+    kernels.synchronize()
+    assert kernels.device_error() == 0
+    # one key each: the output is the value that the cache holds
+    want = expand(*quantise(qkv[:, 32:].astype(np.float64)))
+    assert np.array_equal(d_out.download(np.float16, (tokens, 16, 128)), want.astype(np.float16))
+
+
+@gpu
 def test_host_pointers_are_refused():
     host = torch.zeros(16, 8, 64, dtype=torch.float16)
     dev = host.cuda()
