@@ -22,7 +22,8 @@ namespace cn {
 
 // Device error word (first error wins).  Codes:
 //   1 TMA-full wait timeout, 2 smem-empty wait timeout, 3 MMA-done wait timeout,
-//   4 bad launch shape seen on device, 5 TMEM alloc returned unexpected base.
+//   4 bad launch shape seen on device, 5 TMEM alloc returned unexpected base,
+//   6 a page table entry names no page of the cache, or a position lies past the table.
 __device__ int g_cn_dev_error = 0;  // the library is built as one translation unit (cn_lib.cu)
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s

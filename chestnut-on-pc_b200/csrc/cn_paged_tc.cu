@@ -421,19 +421,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           if (h == 0) {  // its V is in order, and what lies beside it
             if (!many_wait(&bar.vfix[st], (fixes >> st) & 1, 2)) return false;
           }
-          // what a row does not see becomes -inf in tensor memory; all else goes on as everywhere
-          const int k0 = p.lo + j * kManyKeys + h * 64, clo = see_lo - k0, chi = see_hi - k0;
-#pragma unroll 1
-          for (int c0 = 0; c0 < 64; c0 += 32) {
-            uint32_t y[32];
-            tmem_ld32(th + c0, y);
-            tmem_ld_wait32(y);
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (c0 + c < clo || c0 + c >= chi) y[c] = 0xff800000u;
-            tmem_st32(th + c0, y);
-          }
-          tmem_st_wait();
         }
         if constexpr (CODED) {
           if (h == 0) {
@@ -446,6 +433,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           tmem_ld32(th + 32, s1);
           tmem_ld_wait32(s0);
           tmem_ld_wait32(s1);
+          if constexpr (EDGE) {  // what a row does not see
+            const int k0 = p.lo + j * kManyKeys + h * 64, clo = see_lo - k0, chi = see_hi - k0;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              if (c < clo || c >= chi) s0[c] = 0xff800000u;
+              if (c + 32 < clo || c + 32 >= chi) s1[c] = 0xff800000u;
+            }
+          }
           if constexpr (CODED) {
             const uint64_t rs2 = pair2(rs, rs);
             auto to_powers = [&](uint32_t* y, int c0) {
