@@ -71,7 +71,7 @@ struct ManyBars {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4], vfix[4];  // stages
   uint64_t sfull[2][2], pfull[2][2];                           // [half][64 keys of a block]
   uint64_t odone[2][2];                                        // its product with V is added to O
-  uint64_t asked;                                              // V of an edge block is on its way
+  uint64_t asked[4];                                           // stages: V of an edge block is on its way
   uint64_t qfull, qempty;
   uint64_t told[2], heard[2];                                  // parts: worked out, read by all
   uint64_t joined;                                             // both halves' sums of a dual part are out
@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       mbar_init(&bar.kempty[i], 2);
       mbar_init(&bar.vempty[i], 2);
       mbar_init(&bar.vfix[i], 128);
+      mbar_init(&bar.asked[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.drain[i], 1);
@@ -345,7 +346,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     mbar_init(&bar.joined, 256);
     mbar_init(&bar.qfull, 128);
     mbar_init(&bar.qempty, 2);
-    mbar_init(&bar.asked, 1);
     fence_barrier_init();
     if (a.q_map) tma_prefetch_desc(&tm_q);
     if constexpr (!CODED) {
@@ -695,7 +695,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     // ------------------------------------------------------------ loads
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Load));
     const int lt = tid - 256;
-    uint32_t nb = 0, np = 0, edges = 0;  // blocks, parts with blocks, edge blocks so far
+    uint32_t nb = 0, np = 0, edges = 0;  // blocks, parts with blocks so far; phase bits of `asked`
     bool ok = true;
     const int shift = a.b.page_shift, page_rows = 1 << shift;
     const int box_rows = min(page_rows, kManyKeys);
@@ -885,12 +885,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
         }
         if (edge && ok) {
-          // the other warps come here ahead of the one that asks for V: a parity says
-          // nothing about a block that is not asked for yet
+          // The other warps come here ahead of the one that asks for V, or after it has gone on: a
+          // parity tells a phase from the next one only.  So the word that V is asked for goes by
+          // stage: a stage's next block waits for this fix, that is, for all four warps.
           if constexpr (!CODED) {
-            if (lt == 32) mbar_arrive(&bar.asked);
-            ok = __all_sync(0xffffffffu, mbar_wait(&bar.asked, edges & 1, 2));  // asleep: three warps wait here long
-            ++edges;
+            if (lt == 32) mbar_arrive(&bar.asked[st]);
+            ok = __all_sync(0xffffffffu, mbar_wait(&bar.asked[st], (edges >> st) & 1, 2));  // asleep: it can take long
+            edges ^= 1u << st;
             if (!ok) break;
           }
           ok = many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1);

@@ -415,6 +415,11 @@ LARGE = [
     ("bf16", "bf16", 64, 32, 3, 5, [255, 256, 257], [129, 127, 128], True, 128),
     ("f16", "f16", 128, 64, 1, 1, [129, 128, 127, 1], [640, 64, 0, 0], False, 0),
     ("f16", "f16", 64, 16, 2, 2, [1] * 300 + [40], list(range(300)) + [1000], True, 0),
+    # many blocks at the edge one after the other, of all stages
+    ("f16", "f16", 64, 32, 4, 3, [701, 5, 300, 64, 400], [0, 5000, 2000, 700, 3000], True, 500),
+    ("bf16", "bf16", 128, 32, 4, 1, [701, 5, 300, 64, 400], [0, 5000, 2000, 700, 3000], True, 300),
+    ("f16", "f16", 128, 16, 4, 2, [500, 130, 257], [0, 1000, 5], True, 120),
+    ("f16", "f16", 64, 64, 8, 1, [900, 33], [50, 700], True, 64),
 ]
 
 
