@@ -318,8 +318,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __shared__ ManyPart parts[2];
   __shared__ float2 join_ml[2][2][128];                 // (m, l) of a dual part's halves (such parts in turn)
   __shared__ uint32_t bad[L::Stages][4];                        // V rows of an edge block that are not finite
-  // 8-bit cache, of each pair of keys: {scale 2^ek, scale 2^ek'}, {ev, ev'}; and {2^-ev, 2^-ev'}
-  __shared__ __align__(16) float kvx[CODED ? L::Stages : 1][CODED ? 64 : 1][2][2];
+  // 8-bit cache, of each pair of keys: {scale 2^ek, scale 2^ek'}, as deep again as K's ring (a
+  // block's softmax reads them when its K's stage is free already), {ev, ev'} and {2^-ev, 2^-ev'}
+  __shared__ __align__(16) float kscale[CODED ? 2 * L::Stages : 1][CODED ? 64 : 1][2];
+  __shared__ __align__(16) float vexp[CODED ? L::Stages : 1][CODED ? 64 : 1][2];
   __shared__ __align__(16) float vback[CODED ? L::Stages : 1][CODED ? 64 : 1][2];
   __shared__ float qpow[2][CODED ? kManyRows : 1];      // power of two that a row of Q was divided by (parts in turn)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -446,10 +448,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             auto to_powers = [&](uint32_t* y, int c0) {
 #pragma unroll
               for (int c = 0; c < 32; c += 2) {
-                const ulonglong2 kv = *reinterpret_cast<const ulonglong2*>(kvx[st][(h * 64 + c0 + c) / 2][0]);
+                const uint64_t ks = *reinterpret_cast<const uint64_t*>(kscale[n % (2 * L::Stages)][(h * 64 + c0 + c) / 2]);
+                const uint64_t ve = *reinterpret_cast<const uint64_t*>(vexp[st][(h * 64 + c0 + c) / 2]);
                 uint64_t v = pair2(y[c], y[c + 1]);
                 if constexpr (std::is_same_v<T, __nv_bfloat16>) v = mul2(v, rs2);
-                const float2 f = unpair2(fma2(v, kv.x, kv.y));
+                const float2 f = unpair2(fma2(v, ks, ve));
                 y[c] = __float_as_uint(f.x);
                 y[c + 1] = __float_as_uint(f.y);
               }
@@ -507,7 +510,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
               if (!((bad[st][2 * h + (c >> 5)] >> (c & 31)) & 1u)) continue;
               float w = __uint_as_float(tmem_ld1(th + c));
               if constexpr (CODED)
-                w = exp2_approx(fmaf(w * rs, kvx[st][(h * 64 + c) >> 1][0][c & 1], kvx[st][(h * 64 + c) >> 1][1][c & 1]) + sub);
+                w = exp2_approx(fmaf(w * rs, kscale[n % (2 * L::Stages)][(h * 64 + c) >> 1][c & 1], vexp[st][(h * 64 + c) >> 1][c & 1]) + sub);
               else
                 w = exp2_approx(fmaf(w, a.scale, sub));
               const int key = p.lo + j * kManyKeys + h * 64 + c;
@@ -857,19 +860,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint32_t n = nb + i, st = n % L::Stages;
         const bool edge = many_edge(p, j);
         if constexpr (CODED) {
+          // K waits for its stage alone: in a dual part the products of the block whose V lies two
+          // before wait for this K
           if (n >= L::Stages) ok = many_wait(&bar.kempty[st], ((n / L::Stages) & 1) ^ 1, 2);
           if (!ok) break;
-          // kvx and vback of a stage are read by the softmax of its block, which is over when its
-          // products with V are: kempty alone would not say so
-          if (n >= L::Stages) ok = many_wait(&bar.vempty[st], ((n / L::Stages) & 1) ^ 1, 2);
-          if (!ok) break;
           put(ck, sk + st * L::Tile);
-          kvx[st][lt >> 1][0][lt & 1] = exp_byte(ek) * a.scale;
+          kscale[n % (2 * L::Stages)][lt >> 1][lt & 1] = exp_byte(ek) * a.scale;
           fence_proxy_async_smem();
           mbar_arrive(&bar.kfull[st]);
           if (i + 1 < blocks) ek = hold(j + 1, page, a.k, a.k_exp, ck);
+          if (n >= L::Stages) ok = many_wait(&bar.vempty[st], ((n / L::Stages) & 1) ^ 1, 2);
+          if (!ok) break;
           put(cv, sv + st * L::Tile);
-          kvx[st][lt >> 1][1][lt & 1] = (float)((int)ev - 127);
+          vexp[st][lt >> 1][lt & 1] = (float)((int)ev - 127);
           vback[st][lt >> 1][lt & 1] = exp_byte(254u - ev);
           fence_proxy_async_smem();
           mbar_arrive(&bar.vfull[st]);

@@ -415,6 +415,12 @@ LARGE = [
     ("bf16", "bf16", 64, 32, 3, 5, [255, 256, 257], [129, 127, 128], True, 128),
     ("f16", "f16", 128, 64, 1, 1, [129, 128, 127, 1], [640, 64, 0, 0], False, 0),
     ("f16", "f16", 64, 16, 2, 2, [1] * 300 + [40], list(range(300)) + [1000], True, 0),
+    # tiles of one half over several blocks of keys an SM, each cache and dim
+    ("f16", "e4m3", 128, 64, 4, 3, list(range(17, 42)), [459] * 25, True, 0),
+    ("bf16", "e4m3", 128, 16, 8, 1, [40] * 16, [900 + 61 * i for i in range(16)], False, 0),
+    ("bf16", "bf16", 128, 64, 4, 3, list(range(17, 42)), [459] * 25, True, 0),
+    ("f16", "e4m3", 64, 64, 8, 3, list(range(17, 42)), [1459] * 25, True, 700),
+    ("f16", "f16", 64, 64, 8, 3, list(range(17, 42)), [1459] * 25, True, 0),
     # many blocks at the edge one after the other, of all stages
     ("f16", "f16", 64, 32, 4, 3, [701, 5, 300, 64, 400], [0, 5000, 2000, 700, 3000], True, 500),
     ("bf16", "bf16", 128, 32, 4, 1, [701, 5, 300, 64, 400], [0, 5000, 2000, 700, 3000], True, 300),
