@@ -49,13 +49,16 @@ constexpr int kManyKeys = 128;
 constexpr int kManyThreads = 512;
 constexpr float kLazy = 8.f;  // the maximum may be exceeded by 2^8 before it is raised
 
-// Registers of the warpgroups (softmax, loads, products): their sum is 4 x 128, what the block is launched with.
+// Registers of the warpgroups (softmax, loads, products): their sum is 4 x 128, what the block is
+// launched with.  setmaxnreg.dec to more than 128 would be an illegal instruction.  Over an 8-bit
+// cache the loads hold two blocks' codes: with 96 registers they spilled (dim 128, chunks of up to
+// 701 tokens: 350 us, 263 us with 128).
 template <bool CODED>
 struct ManyRegs {
-  static constexpr int Softmax = CODED ? 176 : 192;
-  static constexpr int Load = CODED ? 96 : 64;
+  static constexpr int Softmax = CODED ? 160 : 192;
+  static constexpr int Load = CODED ? 128 : 64;
   static constexpr int Mma = 64;
-  static_assert(2 * Softmax + Load + Mma == 512, "register split");
+  static_assert(2 * Softmax + Load + Mma == 512 && Softmax >= 128 && Load <= 128 && Mma <= 128, "register split");
 };
 
 template <int DIM>
@@ -430,153 +433,153 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             if (!many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1)) return false;
           }
         }
-          uint32_t s0[32], s1[32];
-          tmem_ld32(th, s0);
-          tmem_ld32(th + 32, s1);
-          tmem_ld_wait32(s0);
-          tmem_ld_wait32(s1);
-          if constexpr (EDGE) {  // what a row does not see
-            const int k0 = p.lo + j * kManyKeys + h * 64, clo = see_lo - k0, chi = see_hi - k0;
+        uint32_t s0[32], s1[32];
+        tmem_ld32(th, s0);
+        tmem_ld32(th + 32, s1);
+        tmem_ld_wait32(s0);
+        tmem_ld_wait32(s1);
+        if constexpr (EDGE) {  // what a row does not see
+          const int k0 = p.lo + j * kManyKeys + h * 64, clo = see_lo - k0, chi = see_hi - k0;
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              if (c < clo || c >= chi) s0[c] = 0xff800000u;
-              if (c + 32 < clo || c + 32 >= chi) s1[c] = 0xff800000u;
-            }
+          for (int c = 0; c < 32; ++c) {
+            if (c < clo || c >= chi) s0[c] = 0xff800000u;
+            if (c + 32 < clo || c + 32 >= chi) s1[c] = 0xff800000u;
           }
-          if constexpr (CODED) {
-            const uint64_t rs2 = pair2(rs, rs);
-            auto to_powers = [&](uint32_t* y, int c0) {
+        }
+        if constexpr (CODED) {
+          const uint64_t rs2 = pair2(rs, rs);
+          auto to_powers = [&](uint32_t* y, int c0) {
 #pragma unroll
-              for (int c = 0; c < 32; c += 2) {
-                const uint64_t ks = *reinterpret_cast<const uint64_t*>(kscale[n % (2 * L::Stages)][(h * 64 + c0 + c) / 2]);
-                const uint64_t ve = *reinterpret_cast<const uint64_t*>(vexp[st][(h * 64 + c0 + c) / 2]);
-                uint64_t v = pair2(y[c], y[c + 1]);
-                if constexpr (std::is_same_v<T, __nv_bfloat16>) v = mul2(v, rs2);
-                const float2 f = unpair2(fma2(v, ks, ve));
-                y[c] = __float_as_uint(f.x);
-                y[c + 1] = __float_as_uint(f.y);
-              }
-            };
-            to_powers(s0, 0);
-            to_powers(s1, 32);
-          }
-          float mx[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s0[i]);
-#pragma unroll
-          for (int c = 4; c < 28; c += 8)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s0[c + i]), __uint_as_float(s0[c + 4 + i]));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s0[28 + i]), __uint_as_float(s1[i]));
-#pragma unroll
-          for (int c = 4; c < 28; c += 8)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s1[c + i]), __uint_as_float(s1[c + 4 + i]));
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], __uint_as_float(s1[28 + i]));
-          float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          if constexpr (!CODED) top *= a.scale;
-          const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
-          const uint32_t odd = EDGE ? bad[st][2 * h] | bad[st][2 * h + 1] : 0u;
-          const bool begun = ns > ns0 || h > 0;  // there are sums in O
-          const bool any = __any_sync(0xffffffffu, raise);
-          if (__builtin_expect(begun && (any || odd), 0)) {  // O stands still once the product before this one is added
-            if (!many_wait(&bar.odone[t][h ^ 1], (ns + h + 1) & 1, 3)) return false;
-            tc_fence_after();
-          }
-          if (__builtin_expect(any, 0)) {
-            const float c = raise ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
-            if (raise) m = top;
-            l *= c;
-            if (begun) {
-#pragma unroll 1
-              for (int d = 0; d < DIM; d += 32) {
-                uint32_t o[32];
-                tmem_ld32(to + d, o);
-                tmem_ld_wait32(o);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
-                tmem_st32(to + d, o);
-              }
-            }
-          }
-          const float sub = m == -INFINITY ? 0.f : -m;
-          if (EDGE && odd) {
-            // rows of V that are not finite: for the rows that see them, from the cache itself
-            tmem_st_wait();
-#pragma unroll 1
-            for (int c = 0; c < 64; ++c) {
-              if (!((bad[st][2 * h + (c >> 5)] >> (c & 31)) & 1u)) continue;
-              float w = __uint_as_float(tmem_ld1(th + c));
-              if constexpr (CODED)
-                w = exp2_approx(fmaf(w * rs, kscale[n % (2 * L::Stages)][(h * 64 + c) >> 1][c & 1], vexp[st][(h * 64 + c) >> 1][c & 1]) + sub);
-              else
-                w = exp2_approx(fmaf(w, a.scale, sub));
-              const int key = p.lo + j * kManyKeys + h * 64 + c;
-              const bool see = key >= see_lo && key < see_hi;
-              const int page = page_of(a.b, p.seq, key);
-              const long long vr = (((long long)max(page, 0) * a.heads + p.head) << a.b.page_shift) + (key & ((1 << a.b.page_shift) - 1));
-#pragma unroll 1
-              for (int d = 0; d < DIM; d += 32) {
-                uint32_t o[32];
-                tmem_ld32(to + d, o);
-                tmem_ld_wait32(o);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                  float2 v;
-                  if constexpr (CODED)
-                    v = Num<__half>::unpack(codes_to_h2(*reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(a.v) + vr * DIM + d + i)));
-                  else
-                    v = Num<T>::unpack(*reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v) + vr * DIM + d + i));
-                  if (see) {
-                    o[i] = __float_as_uint(fmaf(w, v.x, __uint_as_float(o[i])));
-                    o[i + 1] = __float_as_uint(fmaf(w, v.y, __uint_as_float(o[i + 1])));
-                  }
-                }
-                tmem_st32(to + d, o);
-              }
-              tmem_st_wait();
-            }
-          }
-          uint64_t sum[2] = {0ull, 0ull};
-          const uint64_t scale2 = pair2(CODED ? 1.f : a.scale, CODED ? 1.f : a.scale), sub2 = pair2(sub, sub);
-          uint32_t pk[32];
-          // 16 values at a time: independent of one another, so that the exponentials follow each other closely
-          auto weigh = [&](const uint32_t* y, uint32_t* w, int c0) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 16) {
-              float2 e[8];
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint64_t v = pair2(y[c + 2 * i], y[c + 2 * i + 1]);
-                e[i] = unpair2(CODED ? add2(v, sub2) : fma2(v, scale2, sub2));
-              }
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                e[i].x = exp2_approx(e[i].x);
-                e[i].y = exp2_approx(e[i].y);
-              }
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint64_t v = pair2(e[i].x, e[i].y);
-                if constexpr (CODED)
-                  sum[i & 1] = fma2(v, *reinterpret_cast<const uint64_t*>(vback[st][(h * 64 + c0 + c) / 2 + i]), sum[i & 1]);
-                else
-                  sum[i & 1] = add2(v, sum[i & 1]);
-                w[c / 2 + i] = Num<M>::pack(e[i].x, e[i].y);
-              }
+            for (int c = 0; c < 32; c += 2) {
+              const uint64_t ks = *reinterpret_cast<const uint64_t*>(kscale[n % (2 * L::Stages)][(h * 64 + c0 + c) / 2]);
+              const uint64_t ve = *reinterpret_cast<const uint64_t*>(vexp[st][(h * 64 + c0 + c) / 2]);
+              uint64_t v = pair2(y[c], y[c + 1]);
+              if constexpr (std::is_same_v<T, __nv_bfloat16>) v = mul2(v, rs2);
+              const float2 f = unpair2(fma2(v, ks, ve));
+              y[c] = __float_as_uint(f.x);
+              y[c + 1] = __float_as_uint(f.y);
             }
           };
-          weigh(s0, pk, 0);
-          tmem_st16(th, pk);
-          weigh(s1, pk + 16, 32);
-          tmem_st16(th + 16, pk + 16);
-          const float2 sums = unpair2(add2(sum[0], sum[1]));
-          l += sums.x + sums.y;
+          to_powers(s0, 0);
+          to_powers(s1, 32);
+        }
+        float mx[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = __uint_as_float(s0[i]);
+#pragma unroll
+        for (int c = 4; c < 28; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s0[c + i]), __uint_as_float(s0[c + 4 + i]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s0[28 + i]), __uint_as_float(s1[i]));
+#pragma unroll
+        for (int c = 4; c < 28; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mx[i] = max3(mx[i], __uint_as_float(s1[c + i]), __uint_as_float(s1[c + 4 + i]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], __uint_as_float(s1[28 + i]));
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if constexpr (!CODED) top *= a.scale;
+        const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+        const uint32_t odd = EDGE ? bad[st][2 * h] | bad[st][2 * h + 1] : 0u;
+        const bool begun = ns > ns0 || h > 0;  // there are sums in O
+        const bool any = __any_sync(0xffffffffu, raise);
+        if (__builtin_expect(begun && (any || odd), 0)) {  // O stands still once the product before this one is added
+          if (!many_wait(&bar.odone[t][h ^ 1], (ns + h + 1) & 1, 3)) return false;
+          tc_fence_after();
+        }
+        if (__builtin_expect(any, 0)) {
+          const float c = raise ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
+          if (raise) m = top;
+          l *= c;
+          if (begun) {
+#pragma unroll 1
+            for (int d = 0; d < DIM; d += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + d, o);
+              tmem_ld_wait32(o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+              tmem_st32(to + d, o);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.f : -m;
+        if (EDGE && odd) {
+          // rows of V that are not finite: for the rows that see them, from the cache itself
           tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(&bar.pfull[t][h]);
+#pragma unroll 1
+          for (int c = 0; c < 64; ++c) {
+            if (!((bad[st][2 * h + (c >> 5)] >> (c & 31)) & 1u)) continue;
+            float w = __uint_as_float(tmem_ld1(th + c));
+            if constexpr (CODED)
+              w = exp2_approx(fmaf(w * rs, kscale[n % (2 * L::Stages)][(h * 64 + c) >> 1][c & 1], vexp[st][(h * 64 + c) >> 1][c & 1]) + sub);
+            else
+              w = exp2_approx(fmaf(w, a.scale, sub));
+            const int key = p.lo + j * kManyKeys + h * 64 + c;
+            const bool see = key >= see_lo && key < see_hi;
+            const int page = page_of(a.b, p.seq, key);
+            const long long vr = (((long long)max(page, 0) * a.heads + p.head) << a.b.page_shift) + (key & ((1 << a.b.page_shift) - 1));
+#pragma unroll 1
+            for (int d = 0; d < DIM; d += 32) {
+              uint32_t o[32];
+              tmem_ld32(to + d, o);
+              tmem_ld_wait32(o);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float2 v;
+                if constexpr (CODED)
+                  v = Num<__half>::unpack(codes_to_h2(*reinterpret_cast<const uint16_t*>(static_cast<const uint8_t*>(a.v) + vr * DIM + d + i)));
+                else
+                  v = Num<T>::unpack(*reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.v) + vr * DIM + d + i));
+                if (see) {
+                  o[i] = __float_as_uint(fmaf(w, v.x, __uint_as_float(o[i])));
+                  o[i + 1] = __float_as_uint(fmaf(w, v.y, __uint_as_float(o[i + 1])));
+                }
+              }
+              tmem_st32(to + d, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        uint64_t sum[2] = {0ull, 0ull};
+        const uint64_t scale2 = pair2(CODED ? 1.f : a.scale, CODED ? 1.f : a.scale), sub2 = pair2(sub, sub);
+        uint32_t pk[32];
+        // 16 values at a time: independent of one another, so that the exponentials follow each other closely
+        auto weigh = [&](const uint32_t* y, uint32_t* w, int c0) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 16) {
+            float2 e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint64_t v = pair2(y[c + 2 * i], y[c + 2 * i + 1]);
+              e[i] = unpair2(CODED ? add2(v, sub2) : fma2(v, scale2, sub2));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              e[i].x = exp2_approx(e[i].x);
+              e[i].y = exp2_approx(e[i].y);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint64_t v = pair2(e[i].x, e[i].y);
+              if constexpr (CODED)
+                sum[i & 1] = fma2(v, *reinterpret_cast<const uint64_t*>(vback[st][(h * 64 + c0 + c) / 2 + i]), sum[i & 1]);
+              else
+                sum[i & 1] = add2(v, sum[i & 1]);
+              w[c / 2 + i] = Num<M>::pack(e[i].x, e[i].y);
+            }
+          }
+        };
+        weigh(s0, pk, 0);
+        tmem_st16(th, pk);
+        weigh(s1, pk + 16, 32);
+        tmem_st16(th + 16, pk + 16);
+        const float2 sums = unpair2(add2(sum[0], sum[1]));
+        l += sums.x + sums.y;
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bar.pfull[t][h]);
         return true;
       };
       // a dual part's blocks by their stages: even ones are half 0's
@@ -696,7 +699,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
   } else if (warp < 12) {
     // ------------------------------------------------------------ loads
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Load));
+    if constexpr (R::Load < 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R::Load));
     const int lt = tid - 256;
     uint32_t nb = 0, np = 0, edges = 0;  // blocks, parts with blocks so far; phase bits of `asked`
     bool ok = true;
