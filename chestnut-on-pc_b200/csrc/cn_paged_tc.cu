@@ -70,6 +70,21 @@ struct Many {
   static constexpr size_t Smem = 1024 + QBytes + 2 * Stages * Tile;
 };
 
+// A wait knows the parity of a phase, so it is right only where the phase before the awaited one has
+// ended already (else it passes at once) and where the one behind it cannot end before the wait is
+// over.  The second holds everywhere because a stage is given back by its waiting threads alone.  The
+// first:
+//   within a part, and from a part that is not dual to any other: an issuing thread waits for the K, V
+//     and fix of every block in turn, and a stage's phase ends before its block is used again;
+//   within a dual part, and from one to the next: a half's blocks have stages of its own (n % 2 = half);
+//   from a dual part to one that is not: the other half's stages come up, whose last phases this half
+//     has not waited for.  qempty tells of them: a half gives it in a dual part when it has its last
+//     scores (its K was there) and has seen its last V (and fix), and every part begins with a wait for
+//     qfull, which follows both halves' qempty.  (Given with the last scores, as in the other parts, it
+//     would leave the other half's last V on its way: this half's wait for the stage's next V would pass
+//     at once, and the product read what lies there.)
+//   softmax warps: a block's scores were issued after all that its issuing thread had waited for; the
+//     halves of a dual part meet at `joined`, behind their last products.
 struct ManyBars {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4], vfix[4];  // stages
   uint64_t sfull[2][2], pfull[2][2];                           // [half][64 keys of a block]
@@ -990,13 +1005,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           scores(q_lo, 1, stage(n));
           tc_commit(&bar.kempty[stage(n)]);
           tc_commit(&bar.kempty[stage(n)]);
-          if (j + 2 >= p.j1) tc_commit(&bar.qempty);
 #pragma unroll 1
           for (; j < p.j1; j += 2, n += 2) {
             ok = v_there(j, n);
             if (!ok) break;
             if (many_edge(p, j)) fixes ^= 1u << stage(n);
             const bool again = j + 2 < p.j1;
+            // Q is free once the last scores are there, but the word waits for this half's last V as
+            // well: see ManyBars
+            if (!again) tc_commit(&bar.qempty);
 #pragma unroll 1
             for (int h = 0; h < 2; ++h) {
               ok = many_wait1(&bar.pfull[t][h], ns & 1, 3);
@@ -1011,7 +1028,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             if (again) {
               tc_commit(&bar.kempty[stage(n + 2)]);
               tc_commit(&bar.kempty[stage(n + 2)]);
-              if (j + 4 >= p.j1) tc_commit(&bar.qempty);
             }
             tc_commit(&bar.vempty[stage(n)]);
             tc_commit(&bar.vempty[stage(n)]);
