@@ -168,6 +168,9 @@ struct Num<__nv_bfloat16> {
 
 // 2^(byte - 127) of a row's exponent byte; the bytes that cn_kv_write makes are 79 .. 175.
 __device__ __forceinline__ float exp_byte(uint32_t byte) { return __uint_as_float(byte << 23); }
+// 2^(127 - byte), finite for every byte: a masked key's weight, 0, is multiplied by it, and its byte
+// may be anything (255 is no power that a row can have: 0 then).
+__device__ __forceinline__ float inverse_exp_byte(uint32_t byte) { return __uint_as_float((254u - min(byte, 254u)) << 23); }
 
 // Two e4m3 codes (low byte first) to two f16 values: exact, e4m3 is a subset of f16.
 __device__ __forceinline__ uint32_t codes_to_h2(uint32_t codes16) {

@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kFewThreads, CODED ? 3 : 2) k_paged_few(const 
             fa *= ek;
             fb *= ek;
             ev[j][e] = (float)((int)x[16] - 127);
-            back[j][e] = exp_byte(254u - x[16]);
+            back[j][e] = inverse_exp_byte(x[16]);
           }
           sv[j][e] = fmaf(sv[j][e], fa, ev[j][e]);
           sv[j][2 + e] = fmaf(sv[j][2 + e], fb, ev[j][e]);

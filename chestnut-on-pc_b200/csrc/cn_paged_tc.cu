@@ -453,14 +453,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tmem_ld32(th + 32, s1);
         tmem_ld_wait32(s0);
         tmem_ld_wait32(s1);
-        if constexpr (EDGE) {  // what a row does not see
-          const int k0 = p.lo + j * kManyKeys + h * 64, clo = see_lo - k0, chi = see_hi - k0;
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (c < clo || c >= chi) s0[c] = 0xff800000u;
-            if (c + 32 < clo || c + 32 >= chi) s1[c] = 0xff800000u;
-          }
-        }
         if constexpr (CODED) {
           const uint64_t rs2 = pair2(rs, rs);
           auto to_powers = [&](uint32_t* y, int c0) {
@@ -477,6 +469,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           };
           to_powers(s0, 0);
           to_powers(s1, 32);
+        }
+        if constexpr (EDGE) {  // what a row does not see (last: a masked key's powers may be no numbers)
+          const int k0 = p.lo + j * kManyKeys + h * 64, clo = see_lo - k0, chi = see_hi - k0;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            if (c < clo || c >= chi) s0[c] = 0xff800000u;
+            if (c + 32 < clo || c + 32 >= chi) s1[c] = 0xff800000u;
+          }
         }
         float mx[4];
 #pragma unroll
@@ -891,7 +891,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           if (!ok) break;
           put(cv, sv + st * L::Tile);
           vexp[st][lt >> 1][lt & 1] = (float)((int)ev - 127);
-          vback[st][lt >> 1][lt & 1] = exp_byte(254u - ev);
+          vback[st][lt >> 1][lt & 1] = inverse_exp_byte(ev);
           fence_proxy_async_smem();
           mbar_arrive(&bar.vfull[st]);
           if (i + 1 < blocks) ev = hold(j + 1, page, a.v, a.v_exp, cv);

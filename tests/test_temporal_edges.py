@@ -32,3 +32,43 @@ def test_tiles_of_one_and_of_two_halves_in_turn(shape, causal):
     dtype, dim, page, hk, group, seqs = shape
     ops.test_attention_over_long_contexts((dtype, dtype, dim, page, hk, group, [n for n, _ in seqs],
                                            [total - n for n, total in seqs], causal, 0))
+
+
+def unseen(st, first):
+    """Whether each place of the cache [pages][page] holds no key that some row sees (first: of each sequence)."""
+    hidden = np.ones((st["pages"], st["page"]), bool)
+    for s, n in enumerate(st["length"]):
+        for p in range(max(first[s], 0), n):
+            hidden[int(st["table"][s, p // st["page"]]), p % st["page"]] = False
+    return torch.from_numpy(hidden).cuda()
+
+
+@gpu
+@pytest.mark.parametrize("byte", [0, 1, 254, 255])
+@pytest.mark.parametrize("dtype,dim", [("f16", 64), ("f16", 128), ("bf16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("new,past,window", [([1, 1, 2], [4, 100, 33], 0), ([3, 2], [30, 200], 20), ([150], [20], 0),
+                                             ([90, 40], [200, 333], 64)])
+def test_powers_of_two_that_no_row_sees(dtype, dim, byte, new, past, window):
+    """Any exponent byte behind a context's end, in unused pages and in front of the window, beside NaN codes."""
+    st = ops.make(dtype, "e4m3", dim, 16, 2, 2, new, past)
+    hidden = unseen(st, [p - window + 1 if window else 0 for p in past])
+    for m in "kv":
+        st[m].masked_fill_(hidden[:, None, :, None], 0x7f)
+        st[m + "_exp"].masked_fill_(hidden[:, None], byte)
+    out = ops.attend(st, window=window)
+    assert kernels.device_error() == 0
+    ops.check_attention(st, out, window=window)
+
+
+@gpu
+@pytest.mark.parametrize("byte", [0, 255])
+@pytest.mark.parametrize("new,past,window", [([4], [40], 0), ([150], [20], 0), ([90], [200], 64)])
+def test_a_power_of_two_that_one_row_sees(byte, new, past, window):
+    """The newest token's exponent bytes are no numbers: the rows before it do not know."""
+    st = ops.make("f16", "e4m3", 64, 16, 2, 2, new, past)
+    p = st["length"][0] - 1
+    for m in "kv":
+        st[m + "_exp"][int(st["table"][0, p // 16]), :, p % 16] = byte
+    out = ops.attend(st, window=window)
+    out[new[0] - 1] = 7.0  # the row that sees it
+    ops.check_attention(dict(st, new=[new[0] - 1]), out, window=window)
