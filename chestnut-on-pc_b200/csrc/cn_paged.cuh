@@ -76,13 +76,13 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedArgs& a, int s) {
 }
 
 // Tokens of tile b.
-__device__ __forceinline__ int paged_tokens(const PagedArgs& a, const PagedSeq& q, int b) {
+__host__ __device__ __forceinline__ int paged_tokens(const PagedArgs& a, const PagedSeq& q, int b) {
   return min(q.n - b * a.tile_tokens, a.tile_tokens);
 }
 
 // Keys [lo, hi) that tokens [t0, t0 + n) see, lo rounded down to a unit.
 template <int KEYS>
-__device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedSeq& q, int t0, int n, int* lo, int* hi) {
+__host__ __device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedSeq& q, int t0, int n, int* lo, int* hi) {
   const int first = q.past + t0, last = first + n - 1;  // positions
   *hi = last < 0 ? 0 : a.causal ? min(q.len, last + 1) : q.len;
   *lo = a.window > 0 ? max(first - a.window + 1, 0) / KEYS * KEYS : 0;
@@ -90,15 +90,23 @@ __device__ __forceinline__ void paged_range(const PagedArgs& a, const PagedSeq& 
 
 // Blocks of keys of tile b: at least one, so that rows without keys are written too.
 template <int KEYS>
-__device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& q, int b) {
+__host__ __device__ __forceinline__ int paged_blocks(const PagedArgs& a, const PagedSeq& q, int b) {
   int lo, hi;
   paged_range<KEYS>(a, q, b * a.tile_tokens, paged_tokens(a, q, b), &lo, &hi);
   return max((hi - lo + KEYS - 1) / KEYS, 1);
 }
 // Units that it counts.
 template <int KEYS>
-__device__ __forceinline__ int paged_units(const PagedArgs& a, const PagedSeq& q, int b) {
+__host__ __device__ __forceinline__ int paged_units(const PagedArgs& a, const PagedSeq& q, int b) {
   return paged_blocks<KEYS>(a, q, b) + a.extra;
+}
+// Units of every 32nd tile of one head, from tile `lane` on.  A tile's fit 32 bits (2^30 keys); those of
+// a head grow with the square of a prompt: 10^6 tokens in tiles of two are 2^32.
+template <int KEYS>
+__host__ __device__ __forceinline__ long long paged_lane_units(const PagedArgs& a, const PagedSeq& q, int lane) {
+  long long w = 0;
+  for (int b = lane; b < q.tiles; b += 32) w += paged_units<KEYS>(a, q, b);
+  return w;
 }
 // Block at which unit `at` of the line begins, in a tile from `first` on with n blocks.
 __device__ __forceinline__ int paged_block_at(const PagedArgs& a, long long at, long long first, int n) {
@@ -134,7 +142,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* scratch,
 template <int THREADS>
 struct PagedScratch {
   long long warp_sum[THREADS / 32];
-  int seq_units[THREADS];       // units of one head of a sequence
+  long long seq_units[THREADS];  // units of one head of a sequence
   long long seq_at[2], seq_each[2];
   PagedCut cut[2];
 };
@@ -143,7 +151,7 @@ struct PagedScratch {
 // takes a sequence and its lanes the tiles, a thread where a sequence has one
 // tile at most.
 template <int KEYS, int THREADS>
-__device__ __forceinline__ int paged_count(const PagedArgs& a, int s0, PagedScratch<THREADS>* sc) {
+__device__ __forceinline__ long long paged_count(const PagedArgs& a, int s0, PagedScratch<THREADS>* sc) {
   const int tid = threadIdx.x, lane = tid & 31;
   const int n = min(a.b.n_seqs - s0, THREADS);
   if (a.rows_max <= a.tile_tokens * a.group) {
@@ -153,8 +161,7 @@ __device__ __forceinline__ int paged_count(const PagedArgs& a, int s0, PagedScra
   }
   for (int i = tid >> 5; i < n; i += THREADS / 32) {
     const PagedSeq q = paged_seq(a, s0 + i);
-    int w = 0;
-    for (int b = lane; b < q.tiles; b += 32) w += paged_units<KEYS>(a, q, b);
+    long long w = paged_lane_units<KEYS>(a, q, lane);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
     if (lane == 0) sc->seq_units[i] = w;
@@ -174,12 +181,11 @@ __device__ __forceinline__ long long paged_share(long long total, int c, int n) 
 template <int KEYS, int THREADS>
 __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScratch<THREADS>* sc) {
   const int tid = threadIdx.x, lane = tid & 31;
-  long long total = 0, before = 0, at = 0;
-  int each = 0;
+  long long total = 0, before = 0, at = 0, each = 0;
   for (int s0 = 0; s0 < a.b.n_seqs; s0 += THREADS) {
     long long all;
     each = paged_count<KEYS, THREADS>(a, s0, sc);
-    at = block_scan<THREADS>((long long)a.heads * each, sc->warp_sum, &all);
+    at = block_scan<THREADS>(a.heads * each, sc->warp_sum, &all);
     total += all;
   }
   // CTAs that take part: each has min_units units or more
@@ -198,12 +204,12 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
     if (a.b.n_seqs > THREADS) {  // else the only pass's results are still at hand
       long long all;
       each = paged_count<KEYS, THREADS>(a, s0, sc);
-      at = before + block_scan<THREADS>((long long)a.heads * each, sc->warp_sum, &all);
+      at = before + block_scan<THREADS>(a.heads * each, sc->warp_sum, &all);
       before += all;
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (u[i] >= at && u[i] < at + (long long)a.heads * each) {  // the sequence's thread
+      if (u[i] >= at && u[i] < at + a.heads * each) {  // the sequence's thread
         sc->cut[i].seq = s0 + tid;
         sc->seq_at[i] = at;
         sc->seq_each[i] = each;
@@ -215,10 +221,10 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
     if (k.seq >= 0) {
       const PagedSeq q = paged_seq(a, k.seq);
       const long long rel = u[tid >> 5] - sc->seq_at[tid >> 5];
-      const int each1 = (int)sc->seq_each[tid >> 5];
-      const int head = rel < (1ll << 31) ? (int)((uint32_t)rel / (uint32_t)each1) : (int)(rel / each1);
-      const int in_head = (int)(rel - (long long)head * each1);
-      int begin = 0;  // units of the head before tile b0
+      const long long each1 = sc->seq_each[tid >> 5];
+      const int head = (rel | each1) >> 32 ? (int)(rel / each1) : (int)((uint32_t)rel / (uint32_t)each1);
+      const long long in_head = rel - head * each1;
+      long long begin = 0;  // units of the head before tile b0
       for (int b0 = 0; b0 < q.tiles; b0 += 32) {
         const int n = b0 + lane < q.tiles ? paged_units<KEYS>(a, q, b0 + lane) : 0;
         int x = n;
@@ -231,7 +237,7 @@ __device__ __forceinline__ void paged_find(const PagedArgs& a, int c, PagedScrat
         if (here) {
           k.head = head;
           k.tile = b0 + lane;
-          k.first = sc->seq_at[tid >> 5] + (long long)head * each1 + begin + x - n;
+          k.first = sc->seq_at[tid >> 5] + head * each1 + begin + x - n;
           k.units = n;
           k.start = n - a.extra <= a.snap || u[tid >> 5] - k.first <= a.extra ? k.first : u[tid >> 5];
         }

@@ -72,3 +72,40 @@ def test_a_power_of_two_that_one_row_sees(byte, new, past, window):
     out = ops.attend(st, window=window)
     out[new[0] - 1] = 7.0  # the row that sees it
     ops.check_attention(dict(st, new=[new[0] - 1]), out, window=window)
+
+
+UNITS = """
+#include <cstdio>
+#include <cstdlib>
+#include "%s/cn_paged.cuh"
+int main(int, char** v) {
+  cn::PagedArgs a = {};
+  cn::PagedSeq q = {};
+  a.tile_tokens = atoi(v[1]), a.extra = 2, a.causal = atoi(v[4]), a.window = atoi(v[5]);
+  q.n = atoi(v[2]), q.past = atoi(v[3]), q.len = q.n + q.past;
+  q.tiles = (q.n + a.tile_tokens - 1) / a.tile_tokens;
+  long long sum = 0;
+  for (int lane = 0; lane < 32; ++lane) sum += cn::paged_lane_units<128>(a, q, lane);
+  printf("%%lld %%d %%d", sum, (int)sizeof(cn::paged_lane_units<128>(a, q, 0)), (int)sizeof(cn::PagedScratch<32>::seq_units[0]));
+}
+"""
+
+
+def test_units_of_long_prompts_are_counted_in_64_bits(tmp_path):
+    """The line of work of one head is longer than 2^31 units for prompts that a call may bring."""
+    import subprocess
+    import build
+    src, exe = tmp_path / "units.cu", tmp_path / "units"
+    src.write_text(UNITS % build.CSRC)
+    flags = [f for f in build.FLAGS if f not in ("-v", "-Xptxas", "-O3", "-lineinfo")]
+    subprocess.run([build.NVCC, *flags, str(src), "-o", str(exe)], check=True, capture_output=True)
+    for tile, n, past, causal, window in ((2, 1050001, 0, 1, 0), (32, 4200007, 0, 1, 0), (256, 12000000, 5, 1, 0), (2, 700000, 300000, 0, 0),
+                                          (16, 1000, 77, 1, 300)):
+        t0 = np.arange(0, n, tile, dtype=np.int64)
+        last = past + np.minimum(t0 + tile, n)
+        hi = last if causal else np.full_like(last, past + n)
+        lo = np.maximum(past + t0 - window + 1, 0) // 128 * 128 if window else 0
+        want = int((np.maximum(-(-(hi - lo) // 128), 1) + 2).sum())
+        got = subprocess.run([exe, *map(str, (tile, n, past, causal, window))], check=True, capture_output=True, text=True).stdout
+        assert got == f"{want} 8 8"
+        assert n == 1000 or want >= 1 << 31
