@@ -131,7 +131,7 @@ int paged_check(const char* who, const cn_kv_cache* cache, const cn_kv_batch* ba
     set_last_error("%s: %d query heads read one cache head (at most 128)", who, q->heads / cache->heads);
     return CN_ERR_ARG;
   }
-  if (tokens < 0 || tokens * (q->heads / cache->heads) > (1ll << 30)) {
+  if (tokens < 0 || tokens > (1ll << 30) / (q->heads / cache->heads)) {
     set_last_error("%s: %lld tokens (tokens x query heads of a cache head: at most 2^30)", who, tokens);
     return CN_ERR_ARG;
   }

@@ -109,3 +109,11 @@ def test_units_of_long_prompts_are_counted_in_64_bits(tmp_path):
         got = subprocess.run([exe, *map(str, (tile, n, past, causal, window))], check=True, capture_output=True, text=True).stdout
         assert got == f"{want} 8 8"
         assert n == 1000 or want >= 1 << 31
+
+
+@pytest.mark.parametrize("tokens", [2 ** 28 + 1, 2 ** 62, 2 ** 63 - 1])
+def test_more_rows_than_an_index_holds_are_refused(tokens):
+    q = ops._heads(h=32)
+    L = _lib.lib()
+    assert L.cn_paged_attention(ops._cache(), ops._batch(), q, q, tokens, 0.125, 1, 0, 0x100, 1 << 40, None) == ops.CN_ERR_ARG
+    assert b"2^30" in L.cn_last_error()
