@@ -207,7 +207,12 @@ __global__ void __launch_bounds__(kFewThreads, CODED ? 3 : 2) k_paged_few(const 
                              r < there);
         }
         if constexpr (CODED)
-          if (lane < 2) cp_async16_or_zero(st + 2 * kSlice * RB + lane * 16, (lane ? a.v_exp : a.k_exp) + row, page >= 0);
+          if (lane < 2) {
+            if (page >= 0) cp_async16(ring + (i % ST) * F::Stage + 2 * kSlice * RB + lane * 16, (lane ? a.v_exp : a.k_exp) + row);
+            else  // no page: zeros, times 2^0
+              *reinterpret_cast<uint4*>(ring + (i % ST) * F::Stage + 2 * kSlice * RB + lane * 16) =
+                  make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+          }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };

@@ -733,7 +733,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto look_up = [&](int j) {
         const int k0 = p.lo + j * kManyKeys;
         const int boxes = (min(kManyKeys, p.hi - k0) + box_rows - 1) / box_rows;
-        return j < p.j1 && lane < boxes ? page_of(a.b, p.seq, k0 + lane * box_rows) : -1;
+        if (j >= p.j1 || lane >= boxes) return -1;
+        // a page outside the cache: one behind its last, which TMA fills with zeros
+        const int page = page_of(a.b, p.seq, k0 + lane * box_rows);
+        return page < 0 ? (int)a.b.pages : page;
       };
       auto fetch = [&](int j, int page, uint32_t n, const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty) {
         const uint32_t st = n % L::Stages;

@@ -117,3 +117,29 @@ def test_more_rows_than_an_index_holds_are_refused(tokens):
     L = _lib.lib()
     assert L.cn_paged_attention(ops._cache(), ops._batch(), q, q, tokens, 0.125, 1, 0, 0x100, 1 << 40, None) == ops.CN_ERR_ARG
     assert b"2^30" in L.cn_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,cache", [("f16", "f16"), ("bf16", "bf16"), ("f16", "e4m3"), ("bf16", "e4m3")])
+@pytest.mark.parametrize("dim,page,new,past", [(64, 16, [1, 2], [300, 90]), (128, 64, [150, 40], [600, 300]),
+                                               (64, 128, [20, 300], [900, 100]), (128, 256, [64], [1000]),
+                                               (64, 32, [33, 1, 200], [500, 400, 56])])
+def test_keys_of_pages_outside_the_cache_are_zeros(dtype, cache, dim, page, new, past):
+    """Their K and V read as zeros, in the middle of a context and where a row's keys end, for the rows of both kernels;
+    what other sequences left on the chip does not show."""
+    st = ops.make(dtype, cache, dim, page, 2, 2, new, past, tail_rows=0)
+    for s, n in enumerate(st["length"]):
+        for i, bad in ((n // page // 2, -1), ((n - 1) // page, 2 ** 31 - 1), (0, st["pages"])):
+            if i == 0 and s:
+                continue
+            st["d_table"][s, i] = bad
+            for m in "kv":
+                st["ctx"][m][s][i * page:(i + 1) * page] = 0.0
+    for causal in (True, False):
+        out = ops.attend(st, causal=causal)
+        torch.cuda.synchronize()
+        assert kernels.device_error() == 6
+        ops.check_attention(st, out, causal)
+        assert torch.equal(out, ops.attend(st, causal=causal))
+    torch.cuda.synchronize()
+    assert kernels.device_error() == 6
