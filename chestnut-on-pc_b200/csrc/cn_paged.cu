@@ -188,12 +188,15 @@ __global__ void __launch_bounds__(kFewThreads, CODED ? 3 : 2) k_paged_few(const 
     const int p0 = lo + u0 * kFewKeys + warp * kSlice;
     const int p_end = min(lo + u1 * kFewKeys, hi);  // keys behind it are another part's, or nobody's
     const int n = p_end > p0 ? (p_end - p0 + kFewKeys - 1) / kFewKeys : 0;
-    int next_page = n > 0 ? page_of(a.b, s, p0) : -1;
+    // (what lies in front of every row's window is not looked up: its page may be given up already)
+    const int from = a.window > 0 ? first_pos - a.window + 1 : 0;
+    auto page_at = [&](int pos) { return pos + kSlice > from ? page_of(a.b, s, pos) : -1; };
+    int next_page = n > 0 ? page_at(p0) : -1;
     auto load = [&](int i) {
       if (i < n) {
         const int pos = p0 + i * kFewKeys;
         const int page = next_page;
-        if (i + 1 < n) next_page = page_of(a.b, s, pos + kFewKeys);
+        if (i + 1 < n) next_page = page_at(pos + kFewKeys);
         const long long row = page < 0 ? 0 : (((long long)page * a.heads + head) << a.b.page_shift) + (pos & (page_rows - 1));
         const int there = page < 0 ? 0 : sq.len - pos;  // rows of the slice that exist
         const uint32_t st = ring_u + (i % ST) * F::Stage;

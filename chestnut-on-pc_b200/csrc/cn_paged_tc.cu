@@ -726,6 +726,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       if (lane == 0) part_read();
       if (p.j0 >= p.j1) continue;
       const int blocks = p.j1 - p.j0;
+      // pages that end in front of it are not looked up: no row sees them, and they may be given up already
+      const int from = a.window > 0 ? p.past + p.tok0 - a.window + 1 : 0;
 
       // 16-bit cache: a warp asks for the blocks of K and another one for those of V (whose stages
       // come free later: one warp for both held K back), a lane for a page.  The pages of a block are
@@ -734,8 +736,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const int k0 = p.lo + j * kManyKeys;
         const int boxes = (min(kManyKeys, p.hi - k0) + box_rows - 1) / box_rows;
         if (j >= p.j1 || lane >= boxes) return -1;
-        // a page outside the cache: one behind its last, which TMA fills with zeros
-        const int page = page_of(a.b, p.seq, k0 + lane * box_rows);
+        // no page, or one outside the cache: the one behind its last, which TMA fills with zeros
+        const int key = k0 + lane * box_rows, page = key + box_rows > from ? page_of(a.b, p.seq, key) : -1;
         return page < 0 ? (int)a.b.pages : page;
       };
       auto fetch = [&](int j, int page, uint32_t n, const CUtensorMap* map, uint8_t* ring, uint64_t* full, uint64_t* empty) {
@@ -758,7 +760,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       // (the pages of a block: lane l has that of keys 16 l .. 16 l + 15)
       auto pages = [&](int j) {
         const int key = p.lo + j * kManyKeys + lane * 16;
-        return j < p.j1 && lane < 8 && key < p.hi ? page_of(a.b, p.seq, key) : -1;
+        return j < p.j1 && lane < 8 && key < p.hi && key + 16 > from ? page_of(a.b, p.seq, key) : -1;
       };
       auto hold = [&](int j, int page, const void* cache, const uint8_t* exps, uint4 (&c)[PT]) -> uint32_t {
         const int k0 = p.lo + j * kManyKeys;

@@ -268,7 +268,8 @@ typedef struct cn_kv_cache {
  * are read on the device; a page outside the cache, or a position past
  * table_width pages, is skipped (reads give zeros) and sets the device error
  * word to 6 (cn_device_error).  To the attention the K and V of such a page are
- * zeros, and a context ends with its table. */
+ * zeros, and a context ends with its table; pages that lie wholly in front of
+ * every new token's window are not looked at. */
 typedef struct cn_kv_batch {
   int n_seqs;
   const int *cu_tokens, *lengths, *table;

@@ -143,3 +143,19 @@ def test_keys_of_pages_outside_the_cache_are_zeros(dtype, cache, dim, page, new,
         assert torch.equal(out, ops.attend(st, causal=causal))
     torch.cuda.synchronize()
     assert kernels.device_error() == 6
+
+
+@gpu
+@pytest.mark.parametrize("dtype,cache", [("f16", "f16"), ("bf16", "bf16"), ("f16", "e4m3")])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 32), (128, 128), (64, 256)])
+@pytest.mark.parametrize("new,past,window", [([1, 3], [700, 411], 60), ([1, 1], [640, 1023], 1), ([150], [900], 130),
+                                             ([20, 300], [777, 555], 200)])
+def test_pages_in_front_of_the_window_may_be_given_up(dtype, cache, dim, page, new, past, window):
+    """Table entries of pages that lie wholly in front of every row's window name no page; nothing is reported."""
+    st = ops.make(dtype, cache, dim, page, 2, 2, new, past)
+    for s, p in enumerate(past):
+        st["d_table"][s, : max(0, p - window + 1) // page] = -1
+    out = ops.attend(st, window=window)
+    torch.cuda.synchronize()
+    assert kernels.device_error() == 0
+    ops.check_attention(st, out, window=window)
