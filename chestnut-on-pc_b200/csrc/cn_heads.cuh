@@ -65,9 +65,10 @@ inline int dtype_bytes(int dtype) { return dtype == CN_F32 ? 4 : dtype == CN_E4M
 
 inline bool misaligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
-// Checks of a [tokens][heads][dim] view; `written`: no two of its rows may overlap.
+// Checks of a [tokens][heads][dim] view; `written`: no two of its rows may overlap.  Without tokens it
+// needs no memory (an empty tensor has no address).
 inline int check_heads(const char* who, const char* name, const cn_heads* h, long long tokens, bool written) {
-  if (!h || !h->data) {
+  if (!h || (!h->data && tokens > 0)) {
     set_last_error("%s: %s is missing", who, name);
     return CN_ERR_ARG;
   }

@@ -113,10 +113,12 @@ bool paged_q_map(CUtensorMap* m, const cn_heads* q, long long tokens, int group,
                 b, CU_TENSOR_MAP_SWIZZLE_128B) == 0;
 }
 
+// sizes_only: q's rows need no memory yet.
 int paged_check(const char* who, const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q,
-                long long tokens) {
+                long long tokens, bool sizes_only) {
   int r;
-  if ((r = check_cache(who, cache)) || (r = check_batch(who, batch, cache)) || (r = check_heads(who, "q", q, tokens, false)))
+  if ((r = check_cache(who, cache)) || (r = check_batch(who, batch, cache)) ||
+      (r = check_heads(who, "q", q, sizes_only ? 0 : tokens, false)))
     return r;
   if (q->dtype == CN_F32 || (cache->dtype != CN_E4M3 && cache->dtype != q->dtype)) {
     set_last_error("%s: q has dtype %d, the cache %d (q f16 or bf16, a 16-bit cache the same)", who, q->dtype, cache->dtype);
@@ -149,7 +151,7 @@ extern "C" int cn_paged_attention_workspace(const cn_kv_cache* cache, const cn_k
     set_last_error("%s: bytes is NULL", who);
     return CN_ERR_ARG;
   }
-  const int r = paged_check(who, cache, batch, q, tokens);
+  const int r = paged_check(who, cache, batch, q, tokens, true);
   if (r) return r;
   *bytes = paged_space(kFewCtas, kFewRows, cache->dim).bytes + paged_space(kManyCtas, kManyRows, cache->dim).bytes;
   return 0;
@@ -160,7 +162,7 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
                                   void* workspace, size_t workspace_bytes, void* stream) {
   using namespace cn;
   const char* who = "cn_paged_attention";
-  int r = paged_check(who, cache, batch, q, tokens);
+  int r = paged_check(who, cache, batch, q, tokens, false);
   if (r || (r = check_heads(who, "out", out, tokens, true))) return r;
   if (out->dtype != q->dtype || out->heads != q->heads || out->dim != q->dim) {
     set_last_error("%s: q and out differ in dtype, heads or dim", who);

@@ -141,7 +141,7 @@ extern "C" int cn_rope(const cn_heads* x, const cn_heads* out, long long tokens,
     set_last_error("%s: out starts where x does but has other strides", who);
     return CN_ERR_ARG;
   }
-  if (tokens < 0 || tokens > INT32_MAX || !positions || !inv_freq || reinterpret_cast<uintptr_t>(positions) % 8 ||
+  if (tokens < 0 || tokens > INT32_MAX || (!positions && tokens > 0) || !inv_freq || reinterpret_cast<uintptr_t>(positions) % 8 ||
       reinterpret_cast<uintptr_t>(inv_freq) % 8) {
     set_last_error("%s: tokens out of range, or positions or inv_freq missing or not 8-byte aligned", who);
     return CN_ERR_ARG;

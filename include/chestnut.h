@@ -228,7 +228,8 @@ int cn_decode_frame(cn_engine* e, const cn_decode_field* fields, int n_fields, f
  * calls run on that GPU's stream whatever the current device is; every call
  * only queues work and can be captured into a CUDA graph.  A pointer that is
  * not device memory, or lies on another GPU than the call's first one, is
- * refused. */
+ * refused.  A call without tokens does nothing; its rows (and positions) may be
+ * NULL. */
 #define CN_F16 0
 #define CN_BF16 1
 #define CN_F32 2

@@ -159,3 +159,24 @@ def test_pages_in_front_of_the_window_may_be_given_up(dtype, cache, dim, page, n
     torch.cuda.synchronize()
     assert kernels.device_error() == 0
     ops.check_attention(st, out, window=window)
+
+
+def test_an_empty_step_needs_no_memory():
+    """No tokens: tensors without elements have no address.  With tokens, or where the batch has sequences, what they
+    need is still asked for."""
+    L = _lib.lib()
+    cache, batch, none = ops._cache(), ops._batch(), ops._heads(ptr=None)
+    assert L.cn_rope(none, none, 0, None, 0x90000, 64, 0, 1.0, None) == 0
+    assert L.cn_kv_write(cache, batch, none, none, 0, None) == 0
+    assert L.cn_kv_read(cache, batch, none, none, 0, None) == 0
+    assert L.cn_paged_attention(cache, batch, none, none, 0, 0.125, 1, 0, None, 0, None) == 0
+    nobody = kernels.kv_batch(0, None, None, None, 0)
+    assert L.cn_paged_attention(cache, nobody, none, none, 0, 0.125, 1, 0, None, 0, None) == 0
+    assert kernels.paged_attention_workspace(cache, batch, none, 0) > 0
+    assert kernels.paged_attention_workspace(cache, batch, none, 5) > 0  # only sizes are read
+    for call in (lambda: L.cn_rope(none, none, 1, 0xa0000, 0x90000, 64, 0, 1.0, None),
+                 lambda: L.cn_rope(ops._heads(), ops._heads(), 1, None, 0x90000, 64, 0, 1.0, None),
+                 lambda: L.cn_kv_write(cache, batch, none, ops._heads(), 1, None),
+                 lambda: L.cn_kv_read(cache, batch, ops._heads(), none, 1, None),
+                 lambda: L.cn_paged_attention(cache, batch, none, ops._heads(), 1, 0.125, 1, 0, 0x100, 1 << 40, None)):
+        assert call() == ops.CN_ERR_ARG
