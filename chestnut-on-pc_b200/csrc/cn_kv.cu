@@ -103,9 +103,9 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], uint32_t* byt
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float2 f = Num<T>::unpack(w[i]);
-    if (infinite) {  // x - x is NaN where x is infinite: such a value becomes NaN, not 448
-      f.x += f.x - f.x;
-      f.y += f.y - f.y;
+    if (infinite) {  // such a value becomes NaN, not 448; the others stay as they are, -0 too (their row may have none)
+      f.x = isinf(f.x) ? NAN : f.x;
+      f.y = isinf(f.y) ? NAN : f.y;
     }
     c[i] = floats_to_codes(f.x * inv, f.y * inv);
   }

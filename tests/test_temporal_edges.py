@@ -180,3 +180,24 @@ def test_an_empty_step_needs_no_memory():
                  lambda: L.cn_kv_read(cache, batch, ops._heads(), none, 1, None),
                  lambda: L.cn_paged_attention(cache, batch, none, ops._heads(), 1, 0.125, 1, 0, 0x100, 1 << 40, None)):
         assert call() == ops.CN_ERR_ARG
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_rows_codes_do_not_depend_on_its_neighbours(dtype, dim):
+    """Negative zeros beside rows with infinities and NaN: their codes are the definition's."""
+    n, hk = 6, 8
+    x = torch.randn(n, hk, dim, generator=torch.Generator().manual_seed(1)).to(ops.TYPES[dtype])
+    x[:, :, ::5] = -0.0
+    x[1::2, 3, 1], x[::2, 4, 2], x[2, 6, 3] = math.inf, -math.inf, math.nan
+    st = ops.make(dtype, "e4m3", dim, 16, hk, 1, [n], [0], fill=0.0)
+    d = x.cuda()
+    kernels.kv_write(*ops.descriptors(st), ops.handle(d, dtype), ops.handle(d, dtype), n, ops.stream())
+    codes, exps = ops.quantise(x.double().numpy())
+    at = int(st["table"][0, 0])
+    for m in "kv":
+        got, e = st[m][at, :, :n].cpu().numpy().swapaxes(0, 1), st[m + "_exp"][at, :, :n].cpu().numpy().T
+        nan = (codes & 0x7f) == 0x7f
+        assert np.array_equal(e, exps) and np.array_equal(np.where(nan, codes, got), codes)
+        assert np.all((got[nan] & 0x7f) == 0x7f)
