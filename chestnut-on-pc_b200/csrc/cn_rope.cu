@@ -137,7 +137,8 @@ extern "C" int cn_rope(const cn_heads* x, const cn_heads* out, long long tokens,
     set_last_error("%s: rot_dim %d of heads of %d values (even, 2 to dim)", who, rot_dim, x->dim);
     return CN_ERR_ARG;
   }
-  if (x->data == out->data && (x->token_stride != out->token_stride || x->head_stride != out->head_stride)) {
+  if (x->data == out->data && ((tokens > 1 && x->token_stride != out->token_stride) ||
+                               (x->heads > 1 && x->head_stride != out->head_stride))) {
     set_last_error("%s: out starts where x does but has other strides", who);
     return CN_ERR_ARG;
   }

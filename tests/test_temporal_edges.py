@@ -201,3 +201,17 @@ def test_a_rows_codes_do_not_depend_on_its_neighbours(dtype, dim):
         nan = (codes & 0x7f) == 0x7f
         assert np.array_equal(e, exps) and np.array_equal(np.where(nan, codes, got), codes)
         assert np.all((got[nan] & 0x7f) == 0x7f)
+
+
+@gpu
+def test_rope_of_one_token_in_place():
+    """One token's or one head's stride says nothing: x and out are the same memory whatever it is."""
+    freq, _ = kernels.rope_frequencies(64)
+    d_freq, pos = torch.from_numpy(freq).cuda(), torch.tensor([5, 9]).cuda()
+    for tokens, h, other in ((1, 4, dict(token_stride=4096)), (2, 1, dict(token_stride=64, head_stride=512))):
+        x = torch.randn(tokens, h, 64, generator=torch.Generator().manual_seed(3)).half().cuda()
+        want = torch.empty_like(x)
+        kernels.rope(ops.handle(x, "f16"), ops.handle(want, "f16"), tokens, pos.data_ptr(), d_freq.data_ptr(), 64, stream=ops.stream())
+        kernels.rope(ops.handle(x, "f16"), kernels.heads(x.data_ptr(), "f16", h, 64, **other), tokens, pos.data_ptr(),
+                     d_freq.data_ptr(), 64, stream=ops.stream())
+        assert torch.equal(x, want)
