@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t max_pairs<__nv_bfloat16>(uint32_t a, uint32_
 // 16 values of a row to codes; every lane of the row gets the row's exponent byte.
 template <typename T, int LANES>
 __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], uint32_t* byte) {
-  const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+  uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = max_pairs<T>(top, w[i] & 0x7fff7fffu);
@@ -84,12 +84,14 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], uint32_t* byt
   float amax = group_max<LANES>(fmaxf(two.x, two.y));
   // (the warp decides together: group_max below is for all lanes)
   const bool infinite = __any_sync(0xffffffffu, isinf(amax));
-  if (infinite) {  // the largest finite one then
+  if (infinite) {  // the largest finite one then; infinities become NaN (not 448), the other values stay as they are
+    constexpr uint32_t quiet = std::is_same_v<T, __half> ? 0x0200u : 0x0040u;
     amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 f = Num<T>::unpack(w[i]);
       amax = fmaxf(amax, fmaxf(isfinite(f.x) ? fabsf(f.x) : 0.f, isfinite(f.y) ? fabsf(f.y) : 0.f));
+      w[i] |= (isinf(f.x) ? quiet : 0u) | (isinf(f.y) ? quiet << 16 : 0u);
     }
     amax = group_max<LANES>(amax);
   }
@@ -102,11 +104,7 @@ __device__ __forceinline__ uint4 quantise16(const uint4 (&raw)[2], uint32_t* byt
   uint32_t c[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    float2 f = Num<T>::unpack(w[i]);
-    if (infinite) {  // such a value becomes NaN, not 448; the others stay as they are, -0 too (their row may have none)
-      f.x = isinf(f.x) ? NAN : f.x;
-      f.y = isinf(f.y) ? NAN : f.y;
-    }
+    const float2 f = Num<T>::unpack(w[i]);
     c[i] = floats_to_codes(f.x * inv, f.y * inv);
   }
   return make_uint4(c[0] | c[1] << 16, c[2] | c[3] << 16, c[4] | c[5] << 16, c[6] | c[7] << 16);
