@@ -22,12 +22,14 @@
 // 2^(s + ev - m), m the running maximum of s + ev (in powers of two), which puts
 // a row's power of two into the exponent; the sum of the weights themselves is
 // that of 2^(s + ev - m) * 2^-ev in f32.  |ev| <= 48, so it loses nothing above
-// 2^-78 of the largest weight.  K's and V's fragments are read as 16-byte pieces
+// 2^-78 of the largest weight.  A V row far smaller than the largest so far has
+// weights below f16's normal numbers for its power of two alone; what their
+// rounding takes is added in f32 (see kFewLoss).  K's and V's fragments are read as 16-byte pieces
 // of a row, with the order of the head's values permuted alike in q (K) or in
 // the output (V), which the sums do not see.
-// Weights are rounded to 16 bits for the product with V (off by 2^-11 of
-// themselves at most in f16, 2^-8 in bf16: the outputs' own rounding); the sum of weights is
-// that of the unrounded ones.
+// Weights are rounded to 16 bits for the product with V: off by 2^-11 of themselves at
+// most in f16, 2^-8 in bf16 (the outputs' own rounding), f16 ones below 2^-29 of the
+// largest by 2^-40 of it.  The sum of weights is that of the unrounded ones.
 #include "cn_paged.cuh"
 
 namespace cn {
@@ -39,6 +41,16 @@ constexpr int kFewKeys = 64;   // keys of a unit: a slice of 16 for each warp
 constexpr int kFewWarps = 4;
 constexpr int kFewThreads = kFewWarps * 32;
 constexpr int kSlice = 16;
+// f16 weights are 2^15 at most, so they are normal numbers down to 2^-29 of the largest and numbers
+// down to 2^-39; of bf16 ones, whose exponents are f32's, the largest is 1.
+template <typename M>
+struct FewTop {
+  static constexpr float value = std::is_same_v<M, __half> ? 15.f : 0.f;
+};
+// Over an 8-bit cache a weight holds its V row's power of two.  One that is no normal number is off by
+// up to 2^-25 in f16, which stands for 2^-25 / 2^ev of a weight; where that is more than kFewLoss of the
+// row's sum of weights, what the rounding took is added in f32.
+constexpr float kFewLow = 0x1p-14f, kFewLoss = 0x1p-33f;
 
 template <int DIM, bool CODED>
 struct Few {
@@ -336,7 +348,7 @@ __global__ void __launch_bounds__(kFewThreads, CODED ? 3 : 2) k_paged_few(const 
           o[x][3] *= cb;
         }
       }
-      const float sub_a = m_a == -INFINITY ? 0.f : m_a, sub_b = m_b == -INFINITY ? 0.f : m_b;
+      const float sub_a = m_a == -INFINITY ? 0.f : m_a - FewTop<M>::value, sub_b = m_b == -INFINITY ? 0.f : m_b - FewTop<M>::value;
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -346,8 +358,29 @@ __global__ void __launch_bounds__(kFewThreads, CODED ? 3 : 2) k_paged_few(const 
           l_a = fmaf(sv[j][e], back[j][e], l_a);
           l_b = fmaf(sv[j][2 + e], back[j][e], l_b);
         }
+      uint32_t low_keys = 0;  // see kFewLoss
       const uint32_t pf[4] = {Num<M>::pack(sv[0][0], sv[0][1]), Num<M>::pack(sv[0][2], sv[0][3]),
                               Num<M>::pack(sv[1][0], sv[1][1]), Num<M>::pack(sv[1][2], sv[1][3])};
+      if constexpr (CODED) {
+        if (__any_sync(0xffffffffu, fminf(fminf(fminf(sv[0][0], sv[0][1]), fminf(sv[1][0], sv[1][1])),
+                                          fminf(fminf(sv[0][2], sv[0][3]), fminf(sv[1][2], sv[1][3]))) <= kFewLow)) {
+          float sum_a = l_a, sum_b = l_b;
+#pragma unroll
+          for (int x = 1; x <= 2; x <<= 1) {
+            sum_a += __shfl_xor_sync(0xffffffffu, sum_a, x);
+            sum_b += __shfl_xor_sync(0xffffffffu, sum_b, x);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int key = 8 * j + 2 * t4 + (e & 1);
+              const float off = 0x1p-25f * inverse_exp_byte(st[2 * kSlice * RB + 16 + key]);
+              if (sv[j][e] > 0.f && sv[j][e] <= kFewLow && off > kFewLoss * (e < 2 ? sum_a : sum_b)) low_keys |= 1u << key;
+            }
+          low_keys = __reduce_or_sync(0xffffffffu, low_keys);
+        }
+      }
 
       // ---- O += P V
       if constexpr (!CODED) {
@@ -385,20 +418,29 @@ __global__ void __launch_bounds__(kFewThreads, CODED ? 3 : 2) k_paged_few(const 
           mma_16816<M>(o[4 * w + 3], pf, codes_to_h2(lo23 >> 16), codes_to_h2(hi23 >> 16));
         }
       }
-      if (bad) {  // rows of V that are not finite: for the rows that see them, from the cache itself
+      // rows of V that are not finite, for the rows that see them, and what the rounding of weights left out: from the
+      // cache itself
+      if (bad | low_keys) {
 #pragma unroll 1
         for (int x = 0; x < kSlice; ++x) {
-          if (!((bad >> (2 * x)) & 3u)) continue;
+          const bool is_bad = (bad >> (2 * x)) & 3u;
+          if (!is_bad && !((low_keys >> x) & 1u)) continue;
           const int key = pos + x;
           const float w00 = x & 1 ? sv[0][1] : sv[0][0], w01 = x & 1 ? sv[0][3] : sv[0][2];
           const float w10 = x & 1 ? sv[1][1] : sv[1][0], w11 = x & 1 ? sv[1][3] : sv[1][2];
           const int from = (lane & ~3) | ((x & 7) >> 1);
-          const float wa = __shfl_sync(0xffffffffu, x < 8 ? w00 : w10, from);
-          const float wb = __shfl_sync(0xffffffffu, x < 8 ? w01 : w11, from);
+          float wa = __shfl_sync(0xffffffffu, x < 8 ? w00 : w10, from);
+          float wb = __shfl_sync(0xffffffffu, x < 8 ? w01 : w11, from);
           const bool in = key < p_end;
           const bool see_a = in && pos_a >= 0 && !(a.causal && key > pos_a) && !(a.window > 0 && key <= pos_a - a.window);
           const bool see_b = in && pos_b >= 0 && !(a.causal && key > pos_b) && !(a.window > 0 && key <= pos_b - a.window);
-          const long long row = (((long long)page_of(a.b, s, key) * a.heads + head) << a.b.page_shift) + (key & (page_rows - 1));
+          if (!is_bad) {
+            wa -= __half2float(__float2half_rn(wa));
+            wb -= __half2float(__float2half_rn(wb));
+          }
+          const int page = page_of(a.b, s, key);
+          if (page < 0) continue;  // its V is zeros
+          const long long row = (((long long)page * a.heads + head) << a.b.page_shift) + (key & (page_rows - 1));
 #pragma unroll
           for (int y = 0; y < NB; ++y)
 #pragma unroll

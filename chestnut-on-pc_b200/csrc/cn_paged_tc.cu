@@ -35,8 +35,12 @@
 // registers.  V rows there that do not exist are zeroed in shared memory, and
 // rows with NaN or infinities, which 0 * inf would carry into rows that do not
 // see them, leave the product and are added by the threads whose row sees them.
-// An 8-bit cache's powers of two: see cn_paged.cu; the loaders leave them as
-// (2^ek * scale, ev, 2^-ev) of each key.
+// An 8-bit cache's powers of two: K's goes to its scores (2^ek * scale of each key).
+// V's goes into its f16 rows, relative to the largest that the part has met: e4m3
+// codes times 2^-15 .. 2^7 are exact, so the weights are those of the softmax alone
+// and no row's size takes bits of another's.  (With V's power in the weights' exponent
+// a row 2^26 larger than the others took them all.)  Rows outside those 22 powers
+// leave the product like rows that are not finite.
 #include <type_traits>
 #include "cn_paged.cuh"
 
@@ -47,7 +51,18 @@ namespace {
 constexpr int kManyRows = 256;
 constexpr int kManyKeys = 128;
 constexpr int kManyThreads = 512;
-constexpr float kLazy = 8.f;  // the maximum may be exceeded by 2^8 before it is raised
+// The maximum may be exceeded by 2^Lazy before it is raised; weights are relative to it times 2^-Top.
+// f16 weights are 2^15 at most then, normal numbers down to 2^-23 of the maximum's and numbers down to
+// 2^-33; bf16 ones have f32's exponents.
+template <typename M>
+struct ManyTop {
+  static constexpr bool F16 = std::is_same_v<M, __half>;
+  static constexpr float Lazy = F16 ? 6.f : 8.f, Top = F16 ? 9.f : 0.f;
+};
+// 8-bit cache: a row of V goes to f16 times 2^(7 - d), d how many powers of two its own is below the
+// largest so far.  That is exact down to d = 22 (codes x 2^-15); rows below do not go through the tensor
+// core, nor do those above kByteTop: the largest so far counts within what cn_kv_write makes.
+constexpr int kSpread = 22, kByteLow = 79, kByteTop = 175;
 
 // Registers of the warpgroups (softmax, loads, products): their sum is 4 x 128, what the block is
 // launched with.  setmaxnreg.dec to more than 128 would be an illegal instruction.  Over an 8-bit
@@ -318,6 +333,39 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
   return (w & e) == e || (w & (e << 16)) == (e << 16);
 }
 
+// Codes of a block of keys, 16 a piece, piece lt + 128 i of the loading thread lt, to f16 rows in the
+// 128-byte swizzle.  V's rows are multiplied by a power of two or left out (see kSpread), by their
+// exponent bytes (a lane of the warp has those of four keys) and the largest of those.
+template <int DIM, bool IS_V, int PT>
+__device__ __forceinline__ void many_put(const uint4 (&c)[PT], uint8_t* to, int lt, uint32_t bytes, int top) {
+  constexpr int PR = DIM / 16;  // pieces of a row
+#pragma unroll
+  for (int i = 0; i < PT; ++i) {
+    const int row = (lt + 128 * i) / PR, piece = (lt + 128 * i) % PR;
+    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+    uint32_t h[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      h[2 * e] = codes_to_h2(w[e] & 0xffffu);
+      h[2 * e + 1] = codes_to_h2(w[e] >> 16);
+    }
+    if constexpr (IS_V) {
+      const int byte = (__shfl_sync(0xffffffffu, bytes, row >> 2) >> (8 * (row & 3))) & 0xff;
+      const int k = min(max(byte - top, -kSpread), 0) + 7;
+      const uint32_t f = (k > -15 ? (uint32_t)(k + 15) << 10 : 0x0200u) * 0x10001u;  // 2^k twice
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(f));
+        if (byte < top - kSpread || byte > top) h[e] = 0;  // a NaN too
+      }
+    }
+    uint8_t* base = to + (piece >> 2) * (128 * 128) + row * 128;
+    const int ch = (piece & 3) * 2;
+    *reinterpret_cast<uint4*>(base + ((ch ^ (row & 7)) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(base + (((ch + 1) ^ (row & 7)) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
+  }
+}
+
 // T: q and out (and a 16-bit cache).
 template <typename T, int DIM, bool CODED>
 __global__ void __launch_bounds__(kManyThreads, 1)
@@ -337,10 +385,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
   __shared__ float2 join_ml[2][2][128];                 // (m, l) of a dual part's halves (such parts in turn)
   __shared__ uint32_t bad[L::Stages][4];                        // V rows of an edge block that are not finite
   // 8-bit cache, of each pair of keys: {scale 2^ek, scale 2^ek'}, as deep again as K's ring (a
-  // block's softmax reads them when its K's stage is free already), {ev, ev'} and {2^-ev, 2^-ev'}
+  // block's softmax reads them when its K's stage is free already); of a block: what V lacks in shared
+  // memory, as a power of two and as 2^-that (below zero: rows left the product)
   __shared__ __align__(16) float kscale[CODED ? 2 * L::Stages : 1][CODED ? 64 : 1][2];
-  __shared__ __align__(16) float vexp[CODED ? L::Stages : 1][CODED ? 64 : 1][2];
-  __shared__ __align__(16) float vback[CODED ? L::Stages : 1][CODED ? 64 : 1][2];
+  __shared__ float2 vrest[L::Stages];
   __shared__ float qpow[2][CODED ? kManyRows : 1];      // power of two that a row of Q was divided by (parts in turn)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -438,14 +486,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         tc_fence_after();
         const uint32_t th = ts + h * 64;
         if constexpr (EDGE) {
-          if (h == 0) {  // its V is in order, and what lies beside it
+          if (h == 0 && (!CODED || many_edge(p, j))) {  // its V is in order, and what lies beside it
             if (!many_wait(&bar.vfix[st], (fixes >> st) & 1, 2)) return false;
           }
         }
         if constexpr (CODED) {
           if (h == 0) {
             if constexpr (std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][(p.dual ? 0 : t * 128) + r];
-            if (!many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1)) return false;
+            // (a block that is not at the edge has been asked for rows that left the product: V is there)
+            if (EDGE && !many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1)) return false;
           }
         }
         uint32_t s0[32], s1[32];
@@ -459,10 +508,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
               const uint64_t ks = *reinterpret_cast<const uint64_t*>(kscale[n % (2 * L::Stages)][(h * 64 + c0 + c) / 2]);
-              const uint64_t ve = *reinterpret_cast<const uint64_t*>(vexp[st][(h * 64 + c0 + c) / 2]);
               uint64_t v = pair2(y[c], y[c + 1]);
               if constexpr (std::is_same_v<T, __nv_bfloat16>) v = mul2(v, rs2);
-              const float2 f = unpair2(fma2(v, ks, ve));
+              const float2 f = unpair2(mul2(v, ks));
               y[c] = __float_as_uint(f.x);
               y[c + 1] = __float_as_uint(f.y);
             }
@@ -494,8 +542,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], __uint_as_float(s1[28 + i]));
         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        if constexpr (!CODED) top *= a.scale;
-        const bool raise = top > m + kLazy || (m == -INFINITY && top > -INFINITY);
+        float rest = 0.f;
+        if constexpr (CODED) top += rest = vrest[st].x;
+        else top *= a.scale;
+        const bool raise = top > m + ManyTop<M>::Lazy || (m == -INFINITY && top > -INFINITY);
         const uint32_t odd = EDGE ? bad[st][2 * h] | bad[st][2 * h + 1] : 0u;
         const bool begun = ns > ns0 || h > 0;  // there are sums in O
         const bool any = __any_sync(0xffffffffu, raise);
@@ -519,22 +569,23 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
           }
         }
-        const float sub = m == -INFINITY ? 0.f : -m;
+        const float sub = m == -INFINITY ? 0.f : ManyTop<M>::Top - m;
         if (EDGE && odd) {
-          // rows of V that are not finite: for the rows that see them, from the cache itself
+          // rows of V that left the product: for the rows that see them, from the cache itself
           tmem_st_wait();
 #pragma unroll 1
           for (int c = 0; c < 64; ++c) {
             if (!((bad[st][2 * h + (c >> 5)] >> (c & 31)) & 1u)) continue;
             float w = __uint_as_float(tmem_ld1(th + c));
-            if constexpr (CODED)
-              w = exp2_approx(fmaf(w * rs, kscale[n % (2 * L::Stages)][(h * 64 + c) >> 1][c & 1], vexp[st][(h * 64 + c) >> 1][c & 1]) + sub);
+            const int key = p.lo + j * kManyKeys + h * 64 + c;
+            const int page = page_of(a.b, p.seq, key);
+            if (page < 0) continue;  // its V is zeros
+            const bool see = key >= see_lo && key < see_hi;
+            const long long vr = (((long long)page * a.heads + p.head) << a.b.page_shift) + (key & ((1 << a.b.page_shift) - 1));
+            if constexpr (CODED)  // (its own power of two in place of the block's)
+              w = exp2_approx(fmaf(w * rs, kscale[n % (2 * L::Stages)][(h * 64 + c) >> 1][c & 1], (float)((int)a.v_exp[vr] - 127)) + sub);
             else
               w = exp2_approx(fmaf(w, a.scale, sub));
-            const int key = p.lo + j * kManyKeys + h * 64 + c;
-            const bool see = key >= see_lo && key < see_hi;
-            const int page = page_of(a.b, p.seq, key);
-            const long long vr = (((long long)max(page, 0) * a.heads + p.head) << a.b.page_shift) + (key & ((1 << a.b.page_shift) - 1));
 #pragma unroll 1
             for (int d = 0; d < DIM; d += 32) {
               uint32_t o[32];
@@ -558,10 +609,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           }
         }
         uint64_t sum[2] = {0ull, 0ull};
-        const uint64_t scale2 = pair2(CODED ? 1.f : a.scale, CODED ? 1.f : a.scale), sub2 = pair2(sub, sub);
+        const uint64_t scale2 = pair2(CODED ? 1.f : a.scale, CODED ? 1.f : a.scale), sub2 = pair2(sub + rest, sub + rest);
         uint32_t pk[32];
         // 16 values at a time: independent of one another, so that the exponentials follow each other closely
-        auto weigh = [&](const uint32_t* y, uint32_t* w, int c0) {
+        auto weigh = [&](const uint32_t* y, uint32_t* w) {
 #pragma unroll
           for (int c = 0; c < 32; c += 16) {
             float2 e[8];
@@ -578,20 +629,18 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const uint64_t v = pair2(e[i].x, e[i].y);
-              if constexpr (CODED)
-                sum[i & 1] = fma2(v, *reinterpret_cast<const uint64_t*>(vback[st][(h * 64 + c0 + c) / 2 + i]), sum[i & 1]);
-              else
-                sum[i & 1] = add2(v, sum[i & 1]);
+              sum[i & 1] = add2(v, sum[i & 1]);
               w[c / 2 + i] = Num<M>::pack(e[i].x, e[i].y);
             }
           }
         };
-        weigh(s0, pk, 0);
+        weigh(s0, pk);
         tmem_st16(th, pk);
-        weigh(s1, pk + 16, 32);
+        weigh(s1, pk + 16);
         tmem_st16(th + 16, pk + 16);
         const float2 sums = unpair2(add2(sum[0], sum[1]));
-        l += sums.x + sums.y;
+        if constexpr (CODED) l = fmaf(sums.x + sums.y, fabsf(vrest[st].y), l);
+        else l += sums.x + sums.y;
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&bar.pfull[t][h]);
@@ -601,10 +650,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto own = [&](int j) { return j >= ja && j < jb && (!p.dual || ((nb + j - p.j0) & 1) == t); };
       // blocks [i0, i1) are not at the edge
       const int i0 = min(max(p.i0, ja), jb), i1 = min(max(p.i1, i0), jb);
+      // 8-bit cache: rows of V left the product (see kSpread), which is the edge's path too
+      auto left = [&](int j) {
+        const uint32_t n = nb + j - p.j0, st = n % L::Stages;
+        ok = many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1);
+        return ok && vrest[st].y < 0.f;
+      };
 #pragma unroll 1
       for (int j = p.j0; j < p.j1 && ok; ++j) {
-        if (j < i0 || j >= i1) {
-          if (own(j)) {
+        if (j < i0 || j >= i1 || (CODED && own(j) && left(j))) {
+          if (own(j) && ok) {
 #pragma unroll 1
             for (int h = 0; h < 2 && ok; ++h) ok = step(std::true_type(), j, h);
             ++ns;
@@ -619,6 +674,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
           if constexpr (!CODED) {
             ok = step(std::false_type(), j, 0) && step(std::false_type(), j, 1);
           } else {
+            if (left(j)) break;
 #pragma unroll 1
             for (int h = 0; h < 2 && ok; ++h) ok = step(std::false_type(), j, h);
           }
@@ -762,7 +818,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const int key = p.lo + j * kManyKeys + lane * 16;
         return j < p.j1 && lane < 8 && key < p.hi && key + 16 > from ? page_of(a.b, p.seq, key) : -1;
       };
-      auto hold = [&](int j, int page, const void* cache, const uint8_t* exps, uint4 (&c)[PT]) -> uint32_t {
+      auto hold = [&](int j, int page, const void* cache, uint4 (&c)[PT]) {
         const int k0 = p.lo + j * kManyKeys;
 #pragma unroll
         for (int i = 0; i < PT; ++i) {
@@ -773,35 +829,30 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             c[i] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(cache) + kr * DIM + ((lt + 128 * i) % PR) * 16);
           }
         }
-        const int at = __shfl_sync(0xffffffffu, page, lt >> 4);
-        if (at < 0 || k0 + lt >= p.hi) return 127u;
-        return exps[(((long long)at * a.heads + p.head) << shift) + ((k0 + lt) & (page_rows - 1))];
       };
-      auto put = [&](const uint4 (&c)[PT], uint8_t* to) {
-#pragma unroll
-        for (int i = 0; i < PT; ++i) {
-          const int row = (lt + 128 * i) / PR, piece = (lt + 128 * i) % PR;
-          const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-          uint32_t h[8];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            h[2 * e] = codes_to_h2(w[e] & 0xffffu);
-            h[2 * e + 1] = codes_to_h2(w[e] >> 16);
-          }
-          uint8_t* base = to + (piece >> 2) * L::Sub + row * 128;
-          const int ch = (piece & 3) * 2;
-          *reinterpret_cast<uint4*>(base + ((ch ^ (row & 7)) * 16)) = make_uint4(h[0], h[1], h[2], h[3]);
-          *reinterpret_cast<uint4*>(base + (((ch + 1) ^ (row & 7)) * 16)) = make_uint4(h[4], h[5], h[6], h[7]);
-        }
+      // their exponent bytes: a thread's key lt of K; of V every warp has all, four keys a lane
+      auto byte_of = [&](int j, int page, int r, const uint8_t* exps) {
+        return exps + ((((long long)page * a.heads + p.head) << shift) + ((p.lo + j * kManyKeys + r) & (page_rows - 1)));
+      };
+      auto hold_ek = [&](int j, int page) -> uint32_t {
+        const int at = __shfl_sync(0xffffffffu, page, lt >> 4);
+        return at < 0 || p.lo + j * kManyKeys + lt >= p.hi ? 127u : *byte_of(j, at, lt, a.k_exp);
+      };
+      auto hold_ev = [&](int j, int page) -> uint32_t {
+        const int at = __shfl_sync(0xffffffffu, page, lane >> 2);
+        return at < 0 ? 0x7f7f7f7fu : *reinterpret_cast<const uint32_t*>(byte_of(j, at, 4 * lane, a.v_exp));
       };
 
       uint4 ck[PT], cv[PT];
       uint32_t ek = 0, ev = 0;
+      int v_top = kByteLow;  // the largest exponent byte of V so far that some row sees
       int page = -1;
       if constexpr (CODED) {
         page = pages(p.j0);
-        ek = hold(p.j0, page, a.k, a.k_exp, ck);
-        ev = hold(p.j0, page, a.v, a.v_exp, cv);
+        hold(p.j0, page, a.k, ck);
+        ek = hold_ek(p.j0, page);
+        hold(p.j0, page, a.v, cv);
+        ev = hold_ev(p.j0, page);
         page = pages(p.j0 + 1);
       } else {
         if (warp == 8) {
@@ -882,24 +933,49 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const int j = p.j0 + i;
         const uint32_t n = nb + i, st = n % L::Stages;
         const bool edge = many_edge(p, j);
+        uint32_t left = 0;  // 8-bit cache: this warp's rows of V that are not in the product
         if constexpr (CODED) {
           // K waits for its stage alone: in a dual part the products of the block whose V lies two
           // before wait for this K
           if (n >= L::Stages) ok = many_wait(&bar.kempty[st], ((n / L::Stages) & 1) ^ 1, 2);
           if (!ok) break;
-          put(ck, sk + st * L::Tile);
+          many_put<DIM, false>(ck, sk + st * L::Tile, lt, 0, 0);
           kscale[n % (2 * L::Stages)][lt >> 1][lt & 1] = exp_byte(ek) * a.scale;
           fence_proxy_async_smem();
           mbar_arrive(&bar.kfull[st]);
-          if (i + 1 < blocks) ek = hold(j + 1, page, a.k, a.k_exp, ck);
+          if (i + 1 < blocks) {
+            hold(j + 1, page, a.k, ck);
+            ek = hold_ek(j + 1, page);
+          }
           if (n >= L::Stages) ok = many_wait(&bar.vempty[st], ((n / L::Stages) & 1) ^ 1, 2);
           if (!ok) break;
-          put(cv, sv + st * L::Tile);
-          vexp[st][lt >> 1][lt & 1] = (float)((int)ev - 127);
-          vback[st][lt >> 1][lt & 1] = inverse_exp_byte(ev);
+          // the largest power of two of V so far that some row sees: the block's, and each row's way to f16
+          const int k0 = p.lo + j * kManyKeys;
+          int top = 0, low = 255;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = k0 + 4 * lane + e, byte = (ev >> (8 * e)) & 0xff;
+            if (key >= from && key < p.hi) {
+              top = max(top, byte);
+              low = min(low, byte);
+            }
+          }
+          v_top = max(v_top, __reduce_max_sync(0xffffffffu, min(top, kByteTop)));
+          many_put<DIM, true>(cv, sv + st * L::Tile, lt, ev, v_top);
+          // rows that left the product: of all 128 keys, then this warp's 32
+          const bool any = __any_sync(0xffffffffu, top > v_top || low < v_top - kSpread);
+          if (any) {
+            const int mine = (__shfl_sync(0xffffffffu, ev, lt >> 2) >> (8 * (lt & 3))) & 0xff;
+            left = __ballot_sync(0xffffffffu, k0 + lt >= from && k0 + lt < p.hi && (mine < v_top - kSpread || mine > v_top));
+          }
+          if (lane == 0) bad[st][warp - 8] = left;
+          if (lt == 0) vrest[st] = make_float2((float)(v_top - 7 - 127), copysignf(inverse_exp_byte(v_top - 7), any ? -1.f : 1.f));
           fence_proxy_async_smem();
           mbar_arrive(&bar.vfull[st]);
-          if (i + 1 < blocks) ev = hold(j + 1, page, a.v, a.v_exp, cv);
+          if (i + 1 < blocks) {
+            hold(j + 1, page, a.v, cv);
+            ev = hold_ev(j + 1, page);
+          }
           page = pages(j + 2);
         } else {
           if (warp == 8) {
@@ -942,7 +1018,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 *reinterpret_cast<uint4*>(vr + d * L::Sub + ((c + lt) & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           const uint32_t bits = __ballot_sync(0xffffffffu, odd);
-          if (lane == 0) bad[st][warp - 8] = bits;
+          if (lane == 0) bad[st][warp - 8] = bits | left;
           fence_proxy_async_smem();
           mbar_arrive(&bar.vfix[st]);
         }

@@ -315,7 +315,9 @@ int cn_kv_read(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_head
  * Query head h reads cache head h / (q.heads / cache.heads), at most 128 of them one.  q and out alike in
  * dtype (CN_F16 or CN_BF16, the cache's own unless that is CN_E4M3), heads and
  * dim; out may be q; scale positive and finite.  Statistics and sums in f32, the weights enter the product
- * with V in 16 bits.  workspace: cn_paged_attention_workspace() bytes, 256-byte
+ * with V in 16 bits: bf16 over a bf16 cache, else f16, whose smallest weights are off by up to 2^-32 of the
+ * row's sum of weights each.  A row whose visible scores are all minus infinity counts as one that sees nothing.
+ * workspace: cn_paged_attention_workspace() bytes, 256-byte
  * aligned, its content of no matter before and after a call; calls that may run
  * at the same time need one each.  Results do not depend on timing. */
 int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_heads* q, const cn_heads* out,

@@ -215,3 +215,123 @@ def test_rope_of_one_token_in_place():
         kernels.rope(ops.handle(x, "f16"), kernels.heads(x.data_ptr(), "f16", h, 64, **other), tokens, pos.data_ptr(),
                      d_freq.data_ptr(), 64, stream=ops.stream())
         assert torch.equal(x, want)
+
+
+def check_columns(st, out, causal=True):
+    """As check_attention, but a column answers for its own values alone: a weight is off by u(f16) of itself, or, where
+    it is too small for that, by 2^-32 of the largest weight of its row."""
+    got, row = out.cpu().double().numpy(), 0
+    hq, scale = st["hk"] * st["group"], st["dim"] ** -0.5
+    for s, (n, p) in enumerate(zip(st["new"], st["past"])):
+        q = st["qkv"][row:row + n, :hq].double().numpy()
+        for i in range(n):
+            for h in range(hq):
+                hi = p + i + 1 if causal else p + n
+                k, v = (st["ctx"][m][s][:hi, h // st["group"]] for m in "kv")
+                a = k @ q[i, h] * scale
+                w = np.exp(a - a.max())
+                w /= w.sum()
+                ref = w @ v
+                big = (np.abs(k) @ np.abs(q[i, h]) * scale).max()
+                err = 2 * (st["dim"] + 4) * ops.U32 * big + 2.0 ** -21 + hi * ops.U32
+                tol = ops.tiny(st["dtype"]) + ops.u(st["dtype"]) * np.abs(ref) + (ops.u("f16") + err) * (w @ np.abs(v)) \
+                    + hi * 2.0 ** -32 * w.max() * np.abs(v).max(0)
+                bad = ~(np.abs(got[row + i, h] - ref) <= tol * (1 + ops.u(st["dtype"])))
+                assert not bad.any(), (s, i, h, np.argwhere(bad)[:4].tolist(), got[row + i, h][bad][:4], ref[bad][:4], tol[bad][:4])
+        row += n
+
+
+def put_v(st, s, p, x):
+    """Row p of sequence s of the 8-bit cache's V becomes x [hk, dim]."""
+    codes, exps = ops.quantise(x)
+    at = int(st["table"][s, p // st["page"]]), p % st["page"]
+    st["v"][at[0], :, at[1]] = torch.from_numpy(codes).cuda()
+    st["v_exp"][at[0], :, at[1]] = torch.from_numpy(exps).cuda()
+    st["ctx"]["v"][s][p] = ops.expand(codes, exps)
+
+
+SIZES = [
+    # dtype, size of the rows, (position, size, column or None: all) of others; size 0: a row of zeros
+    ("f16", 2.0 ** -8, [(3, 2.0 ** 4, 0)]), ("f16", 2.0 ** -8, [(300, 2.0 ** 12, 7)]), ("f16", 1.0, [(2, 2.0 ** -12, 9)]),
+    ("bf16", 1.0, [(3, 2.0 ** 26, 0)]), ("bf16", 2.0 ** -3, [(3, 2.0 ** 17, 5), (200, 2.0 ** 30, 3)]),
+    ("bf16", 2.0 ** -20, [(70, 2.0 ** 20, 0), (71, 0.0, None)]), ("bf16", 2.0 ** -45, [(40, 2.0 ** 45, 1)]),
+    ("bf16", 2.0 ** -26, [(0, 0.0, None)]), ("bf16", 2.0 ** -36, [(5, 0.0, None), (290, 0.0, None)]),
+    ("bf16", 1.0, [(7, 2.0 ** -20, 2), (250, 2.0 ** -40, 4)]), ("bf16", 2.0 ** 20, [(7, 2.0 ** -20, None), (8, 2.0 ** 45, 3)]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{s[0]}-{math.log2(s[1]):.0f}-" + "-".join(f"{p}:{math.log2(x) if x else 0:.0f}" for p, x, _ in s[2]))
+@pytest.mark.parametrize("dim,group,new,past", [(64, 1, [1], [320]), (128, 2, [3, 1], [309, 400]), (64, 2, [40], [300]),
+                                                (128, 1, [150], [310]), (128, 3, [100], [512])])
+def test_rows_of_very_different_sizes(sizes, dim, group, new, past):
+    """An 8-bit cache whose V rows are powers of two apart, the large ones in one column: the other columns keep their
+    average.  A row with a column of its own keeps that; a row of zeros moves nothing."""
+    dtype, size, others = sizes
+    st = ops.make(dtype, "e4m3", dim, 32, 2, group, new, past)
+    rs = np.random.default_rng(5)
+    for s in range(len(new)):
+        own = [c for _, x, c in others if c is not None and 0 < x < size]
+        for p in range(st["length"][s]):
+            x = rs.standard_normal((2, dim)) * size * 2.0 ** rs.integers(-2, 1)
+            x[:, own] = 0
+            put_v(st, s, p, x)
+        for p, amount, column in others:
+            x = np.zeros((2, dim))
+            if column is not None:
+                x[:, column] = amount
+            else:
+                x[:] = amount * rs.standard_normal((2, dim))
+                x[:, own] = 0
+            put_v(st, s, p, x)
+    out = ops.attend(st)
+    assert kernels.device_error() == 0
+    check_columns(st, out)
+    assert torch.equal(out, ops.attend(st))
+
+
+@gpu
+@pytest.mark.parametrize("cache", ["f16", "e4m3"])
+@pytest.mark.parametrize("new", [1, 20])
+def test_many_small_weights_keep_their_sum(cache, new):
+    """One key that outweighs each of 2,000 others by e^16 = 2^23.1: what those add up to.  Off by the weights' rounding
+    and the output's, u(f16) each, and 2^-14 for all that is in f32 (scores of 23, sums of 2,000 values).  Sequences
+    enough that no context is cut."""
+    seqs, hk = 24, 16
+    st = ops.make("f16", cache, 64, 256, hk, 1, [new] * seqs, [2000 - new] * seqs, fill=0.0, tail_rows=0)
+    st["qkv"].zero_()
+    st["qkv"][:, :hk, 0] = 8.0
+    st["d_qkv"].copy_(st["qkv"])
+    codes, exps = ops.quantise(np.eye(1, 64) * 16.0)     # the heavy key: 8 * 16 / sqrt(64) = 16; the others: 0
+    at = st["table"][:, 0].long().cuda()                 # the first page of each sequence
+    st["k"].zero_()
+    if cache == "e4m3":
+        st["k_exp"].fill_(127), st["v_exp"].fill_(127)
+        st["k"][at, :, 0], st["k_exp"][at, :, 0] = torch.from_numpy(codes[0]).cuda(), int(exps[0])
+        st["v"].fill_(0x38)                              # 1.0
+    else:
+        st["k"][at, :, 0, 0] = 16.0
+        st["v"].fill_(1.0)
+    st["v"][at, :, 0] = 0
+    out = ops.attend(st, causal=False).double()
+    want = 1999 * math.exp(-16.0) / (1 + 1999 * math.exp(-16.0))
+    assert torch.all((out - want).abs() <= (2 * ops.u("f16") + 2.0 ** -14) * want + ops.tiny("f16"))
+
+
+@gpu
+@pytest.mark.parametrize("new", [1, 40, 200])
+def test_a_page_outside_the_cache_beside_large_rows(new):
+    """Its zeros count as rows far smaller than the others, and nothing is read for them."""
+    st = ops.make("bf16", "e4m3", 64, 32, 2, 2, [new], [400], tail_rows=0)
+    rs = np.random.default_rng(1)
+    for p in range(st["length"][0]):
+        put_v(st, 0, p, rs.standard_normal((2, 64)) * 2.0 ** 38)
+    st["d_table"][0, 4] = -1
+    st["d_table"][0, 9] = st["pages"]
+    for m in "kv":
+        for page in (4, 9):
+            st["ctx"][m][0][page * 32:page * 32 + 32] = 0.0
+    out = ops.attend(st)
+    torch.cuda.synchronize()
+    assert kernels.device_error() == 6
+    check_columns(st, out)
