@@ -147,19 +147,27 @@ struct PagedScratch {
   PagedCut cut[2];
 };
 
-// Units of one head of sequence s0 + (this thread), 0 behind the last.  A warp
-// takes a sequence and its lanes the tiles, a thread where a sequence has one
-// tile at most.
+// Units of one head of sequence s0 + (this thread), 0 behind the last.  A thread
+// takes a sequence of one tile at most, a warp one of several, its lanes the
+// tiles.  (A warp for every sequence is a chain of loads for each that a warp has:
+// 512 sequences of one token took the four warps 100 us.)
 template <int KEYS, int THREADS>
 __device__ __forceinline__ long long paged_count(const PagedArgs& a, int s0, PagedScratch<THREADS>* sc) {
+  constexpr int WARPS = THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31;
   const int n = min(a.b.n_seqs - s0, THREADS);
-  if (a.rows_max <= a.tile_tokens * a.group) {
-    if (tid >= n) return 0;
-    const PagedSeq q = paged_seq(a, s0 + tid);
-    return q.tiles ? paged_units<KEYS>(a, q, 0) : 0;
+  const bool by_thread = n > WARPS;
+  if (by_thread) {
+    long long w = 0;
+    if (tid < n) {
+      const PagedSeq q = paged_seq(a, s0 + tid);
+      w = q.tiles > 1 ? -1 : q.tiles ? paged_units<KEYS>(a, q, 0) : 0;
+      sc->seq_units[tid] = w;
+    }
+    if (!__syncthreads_or(w < 0)) return w;
   }
-  for (int i = tid >> 5; i < n; i += THREADS / 32) {
+  for (int i = tid >> 5; i < n; i += WARPS) {
+    if (by_thread && sc->seq_units[i] >= 0) continue;
     const PagedSeq q = paged_seq(a, s0 + i);
     long long w = paged_lane_units<KEYS>(a, q, lane);
 #pragma unroll
