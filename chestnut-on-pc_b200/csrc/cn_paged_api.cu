@@ -210,15 +210,22 @@ extern "C" int cn_paged_attention(const cn_kv_cache* cache, const cn_kv_batch* b
   a.causal = causal != 0;
   a.window = min(window, 1 << 30);  // positions end below it
   // Sequences of up to 16 rows go to the kernel for few rows, the others to the
-  // tensor-core one.  How long each is, only the device knows; a launch that
-  // cannot find work is left out, and where no sequence can have more than 128 rows
-  // (each has a token or more) the first kernel takes them all, in tiles of 16
-  // rows: one such sequence reads its context a few times from L2, which costs
-  // less than a launch that most likely finds nothing (48 sequences of 1 to 4
-  // tokens: 167 -> 151 us).
+  // tensor-core one.  How long each is, only the device knows; a launch that cannot
+  // find work is left out.  So is one that costs more than it can give: the first
+  // kernel takes any sequence in tiles of 16 rows, each of which reads the context
+  // from L2, and a second launch that finds nothing costs 11 us (64 tokens of 64
+  // clips over 1000 each, 16 heads x 128 f16: 93 us, with it 105).  It takes all
+  //  - where no sequence can have more than 128 rows, however the tokens are spread
+  //    (two 64-token frames over 300 / 1000 / 4000 / 16000 tokens: 19 / 25 / 47 / 132
+  //    us; both kernels: 26 / 33 / 46 / 82);
+  //  - where none has if each sequence has a token or more, as in a step of one token
+  //    a clip, and the rows are 512 at most.  Where sequences are empty and one has
+  //    all the tokens, that costs (64 slots, a 64-token frame in one, 4 heads a group,
+  //    over the same lengths: 21 / 26 / 49 / 123 us; both: 25 / 28 / 37 / 52), and
+  //    beyond 512 rows more than it saves.
   const long long rows = tokens * a.group;
-  const bool small = batch->n_seqs > 1 && (tokens - batch->n_seqs + 1) * a.group <= 128;
-  const bool steps = a.group <= kFewRows && (tokens <= batch->n_seqs || small);
+  const bool short_all = rows <= 128, short_likely = (tokens - batch->n_seqs + 1) * a.group <= 128 && rows <= 512;
+  const bool steps = batch->n_seqs > 1 && a.group <= kFewRows && (short_all || short_likely);
   PagedCall c;
   memset(&c, 0, sizeof(c));
   c.do_few = batch->n_seqs > 1 ? a.group <= kFewRows : rows <= kFewRows;

@@ -317,6 +317,9 @@ int cn_kv_read(const cn_kv_cache* cache, const cn_kv_batch* batch, const cn_head
  * dim; out may be q; scale positive and finite.  Statistics and sums in f32, the weights enter the product
  * with V in 16 bits: bf16 over a bf16 cache, else f16, whose smallest weights are off by up to 2^-32 of the
  * row's sum of weights each.  A row whose visible scores are all minus infinity counts as one that sees nothing.
+ * Lengths are known on the device alone: a batch of as many sequences as tokens, or more, and up to 512 rows
+ * (tokens times query heads of a cache head) is taken for a step of a token each; where one sequence holds most
+ * of more than 128 rows the result is the same, but slower.
  * workspace: cn_paged_attention_workspace() bytes, 256-byte
  * aligned, its content of no matter before and after a call; calls that may run
  * at the same time need one each.  Results do not depend on timing. */

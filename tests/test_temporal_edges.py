@@ -335,3 +335,15 @@ def test_a_page_outside_the_cache_beside_large_rows(new):
     torch.cuda.synchronize()
     assert kernels.device_error() == 6
     check_columns(st, out)
+
+
+@gpu
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+@pytest.mark.parametrize("group,new", [(1, [64] + [0] * 63), (8, [0] * 40 + [64] + [0] * 23), (4, [64, 64]), (2, [100] + [1] * 99),
+                                       (1, [1] * 600), (4, [0, 1] * 90), (16, [1] * 30 + [9, 0])])
+def test_batches_that_either_kernel_may_take(cache, group, new):
+    """Slots of which one has a frame and the others nothing or a token, two frames, hundreds of single tokens."""
+    st = ops.make("bf16", cache, 64, 16, 1, group, new, [(37 * i) % 150 for i in range(len(new))])
+    out = ops.attend(st)
+    ops.check_attention(st, out)
+    assert torch.equal(out, ops.attend(st)) and kernels.device_error() == 0
