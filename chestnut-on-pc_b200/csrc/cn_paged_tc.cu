@@ -98,8 +98,9 @@ struct Many {
 //     qfull, which follows both halves' qempty.  (Given with the last scores, as in the other parts, it
 //     would leave the other half's last V on its way: this half's wait for the stage's next V would pass
 //     at once, and the product read what lies there.)
-//   softmax warps: a block's scores were issued after all that its issuing thread had waited for; the
-//     halves of a dual part meet at `joined`, behind their last products.
+//   softmax warps: they wait for a block's scores before its V and fix, and the scores were issued after
+//     all that their issuing thread had waited for; the halves of a dual part meet at `joined`, behind
+//     their last products.
 struct ManyBars {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4], vfix[4];  // stages
   uint64_t sfull[2][2], pfull[2][2];                           // [half][64 keys of a block]
@@ -482,7 +483,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto step = [&](auto edge_block, int j, int h) {
         constexpr bool EDGE = decltype(edge_block)::value;
         const uint32_t n = nb + j - p.j0, st = n % L::Stages;
-        if (!many_wait(&bar.sfull[t][h], ns & 1, 3)) return false;
+        if (!CODED || EDGE || h > 0)  // (`left` has waited)
+          if (!many_wait(&bar.sfull[t][h], ns & 1, 3)) return false;
         tc_fence_after();
         const uint32_t th = ts + h * 64;
         if constexpr (EDGE) {
@@ -493,7 +495,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if constexpr (CODED) {
           if (h == 0) {
             if constexpr (std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][(p.dual ? 0 : t * 128) + r];
-            // (a block that is not at the edge has been asked for rows that left the product: V is there)
             if (EDGE && !many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1)) return false;
           }
         }
@@ -650,10 +651,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto own = [&](int j) { return j >= ja && j < jb && (!p.dual || ((nb + j - p.j0) & 1) == t); };
       // blocks [i0, i1) are not at the edge
       const int i0 = min(max(p.i0, ja), jb), i1 = min(max(p.i1, i0), jb);
-      // 8-bit cache: rows of V left the product (see kSpread), which is the edge's path too
+      // 8-bit cache: rows of V left the product (see kSpread), which is the edge's path too.  V is waited
+      // for behind the block's scores, as everywhere: see ManyBars.
       auto left = [&](int j) {
         const uint32_t n = nb + j - p.j0, st = n % L::Stages;
-        ok = many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1);
+        ok = many_wait(&bar.sfull[t][0], ns & 1, 3) && many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1);
         return ok && vrest[st].y < 0.f;
       };
 #pragma unroll 1

@@ -347,3 +347,54 @@ def test_batches_that_either_kernel_may_take(cache, group, new):
     out = ops.attend(st)
     ops.check_attention(st, out)
     assert torch.equal(out, ops.attend(st)) and kernels.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dim,dtype", [(128, "f16"), (64, "bf16")])
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_large_rows_that_come_in_turn(dim, dtype, seed):
+    """An 8-bit cache where one row in fifty is 2^13 larger, so that the power of two of V's blocks changes along a context,
+    over batches whose tiles of one half, pieces of one block and tiles of two halves follow each other on an SM: each
+    call gives the same, and what 64 bits give (of the other columns, and of the large rows' own)."""
+    rng, g = np.random.default_rng(seed), torch.Generator(device="cuda").manual_seed(seed)
+    hk, page, n = 8, 32, 40
+    new = [int(x) for x in rng.choice([0, 1, 36, 64, 64, 50, 17, 64, 200], n)]
+    length = [a + int(b) for a, b in zip(new, rng.choice([0, 20, 50, 600, 650, 1300, 4000], n))]
+    used = [-(-x // page) for x in length]
+    pages, first = sum(used) + 2, np.concatenate([[0], np.cumsum(used)])
+    order = torch.randperm(pages, generator=g, device="cuda").int()
+    table = torch.full((n, max(used)), -1, dtype=torch.int32, device="cuda")
+    for s in range(n):
+        table[s, : used[s]] = order[first[s]:first[s + 1]]
+    st = dict(dtype=dtype, cache="e4m3", dim=dim, page=page, hk=hk, group=1, new=new, pages=pages, width=max(used), d_table=table,
+              d_cu=torch.tensor([0] + np.cumsum(new).tolist(), dtype=torch.int32).cuda(), d_len=torch.tensor(length, dtype=torch.int32).cuda(),
+              d_qkv=torch.randn(sum(new) + 1, hk, dim, generator=g, device="cuda").to(ops.TYPES[dtype]))
+    wide = {}
+    for m in "kv":
+        x = torch.randn(pages, hk, page, dim, generator=g, device="cuda")
+        if m == "v":
+            big = torch.rand(pages, hk, page, 1, generator=g, device="cuda") < 0.02
+            x *= torch.where(big, 2.0 ** 8, 2.0 ** -5)
+            x[..., : dim // 2].masked_fill_(big, 0.0)
+        part, e = torch.frexp(x.abs().amax(-1))
+        e = e - 9 + (part > 0.875).int()
+        codes = torch.ldexp(x, -e[..., None]).to(torch.float8_e4m3fn)
+        st[m], st[m + "_exp"], wide[m] = codes.view(torch.uint8), (e + 127).to(torch.uint8), torch.ldexp(codes.double(), e[..., None])
+    out = ops.attend(st)
+    for _ in range(30):
+        assert torch.equal(out, ops.attend(st))
+    assert kernels.device_error() == 0
+    row = 0
+    for s in range(n):
+        keys = torch.arange(length[s], device="cuda")
+        k, v = (wide[m][table[s].long()[keys // page], :, keys % page].transpose(0, 1) for m in "kv")  # [hk, keys, dim]
+        q = st["d_qkv"][row:row + new[s]].double().transpose(0, 1)
+        a = (q @ k.mT) * dim ** -0.5
+        a.masked_fill_(keys > length[s] - new[s] + torch.arange(new[s], device="cuda")[:, None], -math.inf)
+        w = torch.softmax(a, -1)
+        big = (q.abs() @ k.abs().mT * dim ** -0.5).amax(-1, keepdim=True) if new[s] else 0.0
+        err = 2 * (dim + 4) * ops.U32 * big + 2.0 ** -21 + length[s] * ops.U32
+        tol = ops.tiny(dtype) + ops.u(dtype) * (w @ v).abs() + (ops.u("f16") + err) * (w @ v.abs()) + (w > 0).double() @ v.abs() * 2.0 ** -32
+        off = (out[row:row + new[s]].double().transpose(0, 1) - w @ v).abs() - tol * (1 + ops.u(dtype))
+        assert new[s] == 0 or off.max() <= 0, (s, off.max().item())
+        row += new[s]
