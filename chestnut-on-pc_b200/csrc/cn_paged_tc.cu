@@ -343,7 +343,13 @@ __device__ __forceinline__ void many_put(const uint4 (&c)[PT], uint8_t* to, int 
 #pragma unroll
   for (int i = 0; i < PT; ++i) {
     const int row = (lt + 128 * i) / PR, piece = (lt + 128 * i) % PR;
-    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+    uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w}, f = 0;
+    if constexpr (IS_V) {
+      const int byte = (__shfl_sync(0xffffffffu, bytes, row >> 2) >> (8 * (row & 3))) & 0xff;
+      const int k = min(max(byte - top, -kSpread), 0) + 7;
+      f = (k > -15 ? (uint32_t)(k + 15) << 10 : 0x0200u) * 0x10001u;  // 2^k twice
+      if (byte < top - kSpread || byte > top) w[0] = w[1] = w[2] = w[3] = 0;
+    }
     uint32_t h[8];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -351,14 +357,8 @@ __device__ __forceinline__ void many_put(const uint4 (&c)[PT], uint8_t* to, int 
       h[2 * e + 1] = codes_to_h2(w[e] >> 16);
     }
     if constexpr (IS_V) {
-      const int byte = (__shfl_sync(0xffffffffu, bytes, row >> 2) >> (8 * (row & 3))) & 0xff;
-      const int k = min(max(byte - top, -kSpread), 0) + 7;
-      const uint32_t f = (k > -15 ? (uint32_t)(k + 15) << 10 : 0x0200u) * 0x10001u;  // 2^k twice
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(f));
-        if (byte < top - kSpread || byte > top) h[e] = 0;  // a NaN too
-      }
+      for (int e = 0; e < 8; ++e) asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(h[e]) : "r"(f));
     }
     uint8_t* base = to + (piece >> 2) * (128 * 128) + row * 128;
     const int ch = (piece & 3) * 2;
@@ -483,8 +483,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
       auto step = [&](auto edge_block, int j, int h) {
         constexpr bool EDGE = decltype(edge_block)::value;
         const uint32_t n = nb + j - p.j0, st = n % L::Stages;
-        if (!CODED || EDGE || h > 0)  // (`left` has waited)
-          if (!many_wait(&bar.sfull[t][h], ns & 1, 3)) return false;
+        if (!many_wait(&bar.sfull[t][h], ns & 1, 3)) return false;
         tc_fence_after();
         const uint32_t th = ts + h * 64;
         if constexpr (EDGE) {
@@ -495,6 +494,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if constexpr (CODED) {
           if (h == 0) {
             if constexpr (std::is_same_v<T, __nv_bfloat16>) rs = qpow[np & 1][(p.dual ? 0 : t * 128) + r];
+            // (an inner block has been asked for rows that left the product: its V is there)
             if (EDGE && !many_wait(&bar.vfull[st], (n / L::Stages) & 1, 1)) return false;
           }
         }
@@ -949,8 +949,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             hold(j + 1, page, a.k, ck);
             ek = hold_ek(j + 1, page);
           }
-          if (n >= L::Stages) ok = many_wait(&bar.vempty[st], ((n / L::Stages) & 1) ^ 1, 2);
-          if (!ok) break;
           // the largest power of two of V so far that some row sees: the block's, and each row's way to f16
           const int k0 = p.lo + j * kManyKeys;
           int top = 0, low = 255;
@@ -963,6 +961,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
           }
           v_top = max(v_top, __reduce_max_sync(0xffffffffu, min(top, kByteTop)));
+          if (n >= L::Stages) ok = many_wait(&bar.vempty[st], ((n / L::Stages) & 1) ^ 1, 2);
+          if (!ok) break;
           many_put<DIM, true>(cv, sv + st * L::Tile, lt, ev, v_top);
           // rows that left the product: of all 128 keys, then this warp's 32
           const bool any = __any_sync(0xffffffffu, top > v_top || low < v_top - kSpread);
