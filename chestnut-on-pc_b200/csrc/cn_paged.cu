@@ -9,13 +9,13 @@
 // ring of slices (K and V, cp.async, swizzled against bank conflicts) in shared
 // memory, and has its own running maximum, sum and 16 x DIM accumulator; there
 // is no barrier in the loop.  64 clips of 50 to 8190 tokens, 8 cache heads x 128
-// bf16: 195 us, 5.5 TB/s, 84% of the copy rate.  The 16 query rows of a tile are the M of
+// bf16: 188 us, 5.7 TB/s, 88% of the copy rate.  The 16 query rows of a tile are the M of
 // mma.sync m16n8k16; the tensor work is far below its rate, the unused rows of a
 // single token cost nothing that is short.  The warps' results are joined once a
 // tile part, through shared memory.
 //
 // An 8-bit cache halves the bytes (48 clips of 1200 to 4800 tokens, 16 heads x 128:
-// 155 us, 3.8 TB/s; issue slots are half used and DRAM too: what is left is each
+// 156 us, 3.8 TB/s; issue slots are half used and DRAM too: what is left is each
 // warp's chain of expansion, products and exponentials) and is expanded on the way to the registers:
 // e4m3 codes are f16 values exactly, so the products run in f16, with
 // S = (q . codes_k) * 2^ek and the weights of the codes of V

@@ -12,7 +12,7 @@
 // both products one after the other.  A tile whose tokens fill one half at most
 // gives its odd blocks of keys to the other half (`dual`), which joins its sums
 // in the end.
-// 8192 tokens, causal, 32 heads over 8, 128 bf16: 590 us, 930 TFLOP/s, 56% of the
+// 8192 tokens, causal, 32 heads over 8, 128 bf16: 585 us, 940 TFLOP/s, 56% of the
 // cuBLAS burst rate (at 950 W, near the power cap; 1040 TFLOP/s in short runs).
 // The tensor pipe is 48% busy.  Per 128 keys of 256 rows an SM spends ~4200
 // clocks; the products need 2560 of them (S with N = 64 is bound by shared
@@ -67,7 +67,7 @@ constexpr int kSpread = 22, kByteLow = 79, kByteTop = 175;
 // Registers of the warpgroups (softmax, loads, products): their sum is 4 x 128, what the block is
 // launched with.  setmaxnreg.dec to more than 128 would be an illegal instruction.  Over an 8-bit
 // cache the loads hold two blocks' codes: with 96 registers they spilled (dim 128, chunks of up to
-// 701 tokens: 350 us, 263 us with 128).
+// 701 tokens: a third more time).
 template <bool CODED>
 struct ManyRegs {
   static constexpr int Softmax = CODED ? 160 : 192;
